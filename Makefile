@@ -5,7 +5,8 @@ CSRC  := matryoshka_transcoder_amd/csrc
 SRCS  := $(CSRC)/api.hip $(CSRC)/encode.hip $(CSRC)/select.hip $(CSRC)/decode.hip $(CSRC)/backward.hip $(CSRC)/optim.hip $(CSRC)/aux.hip $(CSRC)/collect.hip $(CSRC)/store.hip $(CSRC)/comm.hip
 OBJS  := $(SRCS:.hip=.o)
 LIB   := matryoshka_transcoder_amd/libmtc.so
-FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result
+# no packed fp32 instructions: the compiler forms them from plain float code, and some of their forms are not reliable here
+FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB)
 

@@ -5,7 +5,7 @@ set -e
 cd "$(dirname "$0")/.."
 NAME=$1; SRC=$2; shift 2
 CS=matryoshka_transcoder_amd/csrc
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 /opt/rocm/bin/hipcc $FLAGS "$@" -c $CS/$SRC.hip -o /tmp/${SRC}_$NAME.o
 OBJS=""
 for f in api encode select decode backward optim aux collect store comm; do
