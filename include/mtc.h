@@ -554,6 +554,46 @@ int mtc_comm_reduce_scatter(mtc_comm* c, const void* send, void* recv, size_t re
 /* recv [world * send_count] = every rank's send [send_count], in rank order */
 int mtc_comm_all_gather(mtc_comm* c, const void* send, void* recv, size_t send_count, int32_t dtype, void* stream);
 
+/* The norms before and after a block of a language model, fused with the block's gate and the residual add (what stands
+ * around a transcoder that replaces a model's MLP; no counterpart in the reference, which leaves them to the model):
+ *     hidden = residual_scale * residual + branch_scale * gate * post(branch)
+ *     normed = pre(hidden)                                    norm(x) = u * (offset + w) + b
+ *     RMS:   u = x / sqrt(mean(x^2) + eps)                    layer: u = (x - mean(x)) / sqrt(var_biased(x) + eps)
+ * in one pass over the rows.  has_branch = 0: normed = pre(residual) alone (branch, gate, hidden NULL, residual_scale 1);
+ * pre_kind = MTC_NORM_NONE: hidden alone; post_kind = MTC_NORM_NONE: the branch is added as it is.
+ * normed is made from the fp32 sum, before hidden's rounding to the model dtype.  All operands in `dtype`; w / b of a norm
+ * may be NULL (scale 1 instead of offset + w, bias 0).  gate: [A] (CHANNEL), one value per row at stride ld_gate (ROW),
+ * [rows][A] (FULL) or one value (SCALAR).  ld_*: row strides in elements, columns are contiguous; 0 repeats one row (inputs).  Any width
+ * 1 .. 8192, stride and alignment; 16-byte accesses when the width is a multiple of 8 and every row starts at a multiple of
+ * 16 bytes, single elements otherwise.  Outputs must not overlap inputs.
+ * stats (optional, float [4][rows]: post mean, post 1/std, pre mean, pre 1/std; only the rows of norms in use are
+ * written) is what the backward needs.  rows = 0 is a no-op. */
+enum { MTC_NORM_NONE = 0, MTC_NORM_RMS = 1, MTC_NORM_LAYER = 2 };
+enum { MTC_GATE_NONE = 0, MTC_GATE_CHANNEL = 1, MTC_GATE_ROW = 2, MTC_GATE_FULL = 3, MTC_GATE_SCALAR = 4 };
+typedef struct mtc_block_norm_desc {
+    int64_t rows;
+    int32_t A, dtype;
+    int32_t has_branch, post_kind, pre_kind, gate_kind;
+    float post_eps, pre_eps, post_offset, pre_offset;
+    float residual_scale, branch_scale;
+    int64_t ld_residual, ld_branch, ld_gate, ld_hidden, ld_normed;
+} mtc_block_norm_desc;
+int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* residual, const void* branch, const void* gate,
+                       const void* post_w, const void* post_b, const void* pre_w, const void* pre_b, void* hidden,
+                       void* normed, float* stats, void* stream);
+/* Gradient of the above from d_hidden (NULL = zero) and d_normed (given exactly when pre_kind is not NONE).  residual, branch,
+ * gate and the weights are the forward's, stats what it left.  Outputs are contiguous, in `dtype`; each may be NULL = not
+ * wanted: d_residual, d_branch [rows][A], d_gate in the gate's own shape ([A] / [rows] / [rows][A] / [1]), the weight and bias
+ * gradients [A] (sums over the rows in fp32, rounded once, the same bits on every run).  workspace:
+ * mtc_block_norm_bwd_workspace_bytes(d), 16-byte aligned, used only for gradients of weights, biases, a channel or a scalar gate.
+ * rows must be > 0. */
+size_t mtc_block_norm_bwd_workspace_bytes(const mtc_block_norm_desc* d);
+int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* residual, const void* branch, const void* gate,
+                       const void* post_w, const void* post_b, const void* pre_w, const void* pre_b, const float* stats,
+                       const void* d_hidden, int64_t ld_d_hidden, const void* d_normed, int64_t ld_d_normed,
+                       void* d_residual, void* d_branch, void* d_gate, void* d_post_w, void* d_post_b, void* d_pre_w,
+                       void* d_pre_b, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

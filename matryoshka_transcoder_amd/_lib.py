@@ -26,10 +26,21 @@ class AdamHyper(C.Structure):
                 ("step", C.c_int32), ("pad", C.c_int32)]
 
 
+class BlockNormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("A", C.c_int32), ("dtype", C.c_int32), ("has_branch", C.c_int32),
+                ("post_kind", C.c_int32), ("pre_kind", C.c_int32), ("gate_kind", C.c_int32), ("post_eps", C.c_float),
+                ("pre_eps", C.c_float), ("post_offset", C.c_float), ("pre_offset", C.c_float),
+                ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("ld_residual", C.c_int64),
+                ("ld_branch", C.c_int64), ("ld_gate", C.c_int64), ("ld_hidden", C.c_int64), ("ld_normed", C.c_int64)]
+
+
+MTC_NORM_NONE, MTC_NORM_RMS, MTC_NORM_LAYER = 0, 1, 2
+MTC_GATE_NONE, MTC_GATE_CHANNEL, MTC_GATE_ROW, MTC_GATE_FULL, MTC_GATE_SCALAR = 0, 1, 2, 3, 4
 SELECT_STATE_BYTES = 64
 P = C.c_void_p
 DP = C.POINTER(Desc)
 HP = C.POINTER(AdamHyper)
+NP = C.POINTER(BlockNormDesc)
 
 # name -> (restype, argtypes); must list every symbol include/mtc.h declares
 PROTOTYPES = {
@@ -118,6 +129,9 @@ PROTOTYPES = {
     "mtc_gather_row_pairs": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, P, P, P, P, P, P, P]),
     "mtc_collect_top_samples": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, P, P, P, P, P, C.c_float,
                                           C.c_int32, C.c_int32, P, P, P, P, P, P, P]),
+    "mtc_block_norm_fwd": (C.c_int, [NP] + [P] * 11),
+    "mtc_block_norm_bwd_workspace_bytes": (C.c_size_t, [NP]),
+    "mtc_block_norm_bwd": (C.c_int, [NP] + [P] * 9 + [C.c_int64, P, C.c_int64] + [P] * 8 + [C.c_size_t, P]),
 }
 
 

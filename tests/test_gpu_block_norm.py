@@ -1,0 +1,361 @@
+"""The block norms on the GPU against a float64 restatement, with tolerances from counted roundings (norm_checks.py)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import norm_checks as N
+from matryoshka_transcoder_amd import _lib
+from matryoshka_transcoder_amd.block_norm import BlockNorm, block_norm, residual_block_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+def _rand(g, *shape, scale=1.0):
+    return torch.randn(shape, generator=g) * scale
+
+
+def _norm_module(g, A, kind, dt, offset=None, affine=True, bias=None):
+    offset = (1.0 if kind == "rms" else 0.0) if offset is None else offset
+    m = BlockNorm(A, kind=kind, eps=1e-6 if kind == "rms" else 1e-5, weight_offset=offset, affine=affine, bias=bias, dtype=dt,
+                  device=DEV)
+    with torch.no_grad():
+        if m.weight is not None:
+            m.weight.copy_(_rand(g, A, scale=0.3) + 1.0 - offset)
+        if m.bias is not None:
+            m.bias.copy_(_rand(g, A, scale=0.2))
+    return m
+
+
+def _spec(m):
+    return None if m is None else dict(w=m.weight, b=m.bias, kind=m.kind, eps=m.eps, off=m.weight_offset)
+
+
+def _gate(g, kind, rows, A, dt):
+    if kind == "none":
+        return None
+    shape = {"scalar": (), "channel": (A,), "token": (rows, 1), "full": (rows, A)}[kind]
+    t = _rand(g, *shape, scale=0.5) + 0.8
+    if kind == "token" and rows > 1:
+        t[::3] = 0.0                                   # tokens kept out of the splice
+    return t.to(dt).to(DEV)
+
+
+def _check(rows, A, dt, mode, post_kind, pre_kind, gate_kind, rs=1.0, bs=1.0, seed=0, edit=None, affine=True, bias=None):
+    g = torch.Generator("cpu").manual_seed(seed * 977 + rows * 31 + A)
+    residual = (_rand(g, rows, A, scale=2.0) + 0.3).to(dt)
+    branch = None if mode == "pre" else (_rand(g, rows, A) - 0.1).to(dt)
+    if edit is not None:
+        edit(residual, branch)
+    residual = residual.to(DEV).requires_grad_(True)
+    branch = None if branch is None else branch.to(DEV).requires_grad_(True)
+    post = _norm_module(g, A, post_kind, dt, affine=affine, bias=bias) if post_kind and mode != "pre" else None
+    pre = _norm_module(g, A, pre_kind, dt, affine=affine, bias=bias) if mode != "post" else None
+    gate = None if mode == "pre" else _gate(g, gate_kind, rows, A, dt)
+    if gate is not None:
+        gate.requires_grad_(True)
+    dh = None if mode == "pre" else _rand(g, rows, A).to(dt).to(DEV)
+    dn = None if mode == "post" else _rand(g, rows, A).to(dt).to(DEV)
+    want = N.reference(residual, branch, gate, _spec(post), _spec(pre), rs, bs, dh, dn)
+    if mode == "pre":
+        outs, names, grads = [pre(residual)], ["normed"], [dn]
+    else:
+        out = residual_block_norm(residual, branch, post, gate=gate, residual_scale=rs, branch_scale=bs, pre=pre)
+        outs, names, grads = ([out], ["hidden"], [dh]) if mode == "post" else (list(out), ["hidden", "normed"], [dh, dn])
+    leaves = {"residual": residual, "branch": branch, "gate": gate, "post_w": post and post.weight, "post_b": post and post.bias,
+              "pre_w": pre and pre.weight, "pre_b": pre and pre.bias}
+    leaves = {k: v for k, v in leaves.items() if v is not None}
+    got = dict(zip(names, outs))
+    got.update(zip(leaves, torch.autograd.grad(outs, list(leaves.values()), grads)))
+    for k, v in got.items():
+        assert v.dtype == dt and v.is_contiguous()
+        N.compare(k, v, want[k], dt)
+    with torch.no_grad():                              # the path without a graph gives the same bits
+        if mode == "pre":
+            again = [pre(residual)]
+        else:
+            out = residual_block_norm(residual, branch, post, gate=gate, residual_scale=rs, branch_scale=bs, pre=pre)
+            again = [out] if mode == "post" else list(out)
+    for a, b in zip(again, outs):
+        assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,A", [(1, 2304), (3, 768), (130, 1600), (257, 2304), (65, 4608), (9, 8192), (1, 8), (70, 64),
+                                    (33, 520), (1, 1), (5, 7), (300, 1001), (2, 8191)])
+def test_pair_rms(rows, A, dt):
+    _check(rows, A, dt, "pair", "rms", "rms", "none")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,A", [(1, 768), (131, 1600), (17, 1283), (40, 4608)])
+@pytest.mark.parametrize("gate", ["none", "scalar", "token", "channel", "full"])
+def test_pair_layer_gates(rows, A, gate, dt):
+    _check(rows, A, dt, "pair", "layer", "layer", gate, rs=0.75, bs=1.5)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("mode,post,pre", [("pre", None, "rms"), ("pre", None, "layer"), ("post", "rms", None), ("post", "layer", None),
+                                           ("post", None, None), ("pair", None, "layer"), ("pair", None, "rms"), ("pair", "rms", "layer"),
+                                           ("pair", "layer", "rms")])
+@pytest.mark.parametrize("gate", ["none", "token", "scalar"])
+def test_modes(mode, post, pre, gate, dt):
+    _check(77, 520, dt, mode, post, pre, gate, rs=1.0 if mode == "pre" else -0.5, bs=0.25)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("affine,bias", [(False, False), (True, False), (True, True)])
+def test_parameters_absent(affine, bias, dt):
+    for kind in ("rms", "layer"):
+        _check(19, 264, dt, "pair", kind, kind, "channel", affine=affine, bias=bias)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_many_rows(dt):
+    _check(5000, 512, dt, "pair", "rms", "layer", "scalar")
+    _check(5003, 2304, dt, "pair", "rms", "rms", "token", seed=3)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rows_far_from_zero_and_empty(dt):
+    def edit(r, b):
+        r[0] = 0
+        b[0] = 0                                       # a row of zeros: eps alone
+        r[1] = 0
+        b[2] = 0
+        r[3] += 64.0                                   # mean far above the spread
+        b[4] -= 64.0
+    for kind in ("rms", "layer"):
+        _check(6, 776, dt, "pair", kind, kind, "none", edit=edit)
+        _check(6, 776, dt, "pair", kind, kind, "token", edit=edit)
+
+
+def test_non_finite_rows_stay_alone():
+    """inf / NaN in a row spoil that row's outputs and the column sums, no other row."""
+    g = torch.Generator("cpu").manual_seed(5)
+    x = _rand(g, 8, 520).to(DEV)
+    x[2, 3], x[5, 100] = float("inf"), float("nan")
+    y = _rand(g, 8, 520).to(DEV)
+    m = _norm_module(g, 520, "rms", torch.float32)
+    hidden, normed = residual_block_norm(x, y, m, pre=m)
+    clean = [0, 1, 3, 4, 6, 7]
+    h2, n2 = residual_block_norm(x[clean], y[clean], m, pre=m)
+    assert torch.equal(hidden[clean], h2) and torch.equal(normed[clean], n2)
+    assert bool(torch.isnan(normed[5]).all()) and not bool(torch.isfinite(normed[2]).all())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_strides_and_alignment(dt):
+    """Row slices of a wider cache, permuted and expanded leading dimensions, strided columns, odd base addresses: the values
+    of the contiguous call (which path serves them is a matter of alignment, so to within the fp32 sums)."""
+    g = torch.Generator("cpu").manual_seed(11)
+    b, s, A = 3, 5, 264
+    post, pre = _norm_module(g, A, "layer", dt), _norm_module(g, A, "rms", dt)
+
+    def run(res, br, gate=None):
+        leaves = [res.detach().requires_grad_(True), br.detach().requires_grad_(True)]
+        with torch.enable_grad():
+            out = residual_block_norm(leaves[0], leaves[1], post, gate=gate, pre=pre)
+            gr = torch.autograd.grad(out, leaves, [torch.ones_like(out[0]), torch.ones_like(out[1])])
+        want = N.reference(res.reshape(-1, A), br.reshape(-1, A), None if gate is None else gate.reshape(-1, gate.shape[-1]), _spec(post),
+                           _spec(pre), 1.0, 1.0, torch.ones(res.numel() // A, A, device=DEV), torch.ones(res.numel() // A, A, device=DEV))
+        for k, v in zip(("hidden", "normed", "residual", "branch"), list(out) + list(gr)):
+            assert tuple(v.shape) == tuple(res.shape)
+            N.compare(k, v, want[k], dt)
+
+    base, base2 = _rand(g, b, s, A).to(dt).to(DEV), _rand(g, b, s, A).to(dt).to(DEV)
+    run(base, base2)
+    wide = _rand(g, b, s, A + 24).to(dt).to(DEV)
+    run(wide[..., 8:8 + A], base2)                                   # aligned rows at a larger stride
+    run(wide[..., 3:3 + A], base2)                                   # rows that no 16-byte access may touch
+    run(base.transpose(0, 1), base2.transpose(0, 1))                 # [s, b, A]
+    run(base[:1].expand(b, s, A), base2)                             # broadcast residual
+    cols = _rand(g, b, s, 2 * A).to(dt).to(DEV)
+    run(cols[..., ::2], base2)                                       # strided columns
+    odd = torch.empty(b * s * A + 1, dtype=dt, device=DEV)[1:].reshape(b, s, A).copy_(base)
+    run(odd, base2)                                                  # base address off by one element
+    run(base[0, 0], base2[0, 0])                                     # one token, one dimension
+    gate = (torch.rand(b, 1, 1, generator=g) > 0.5).to(dt).to(DEV).expand(b, s, 1)
+    run(base, base2, gate)
+    run(base, base2, wide[..., 1:1 + A])
+
+
+def test_expanded_residual_gradient():
+    """A residual broadcast over the batch: its gradient is the sum over the copies."""
+    g = torch.Generator("cpu").manual_seed(12)
+    r = _rand(g, 1, 4, 128).to(DEV).requires_grad_(True)
+    y = _rand(g, 3, 4, 128).to(DEV)
+    (gr,) = torch.autograd.grad(residual_block_norm(r.expand(3, 4, 128), y, None).sum(), [r])
+    assert gr.shape == r.shape and torch.equal(gr, torch.full_like(gr, 3.0))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_partial_gradients(dt):
+    """Only what is asked for: one incoming gradient, frozen norms, a branch without gradient."""
+    g = torch.Generator("cpu").manual_seed(13)
+    rows, A = 40, 520
+    res, br = _rand(g, rows, A).to(dt).to(DEV), _rand(g, rows, A).to(dt).to(DEV)
+    post, pre = _norm_module(g, A, "rms", dt), _norm_module(g, A, "layer", dt)
+    d = _rand(g, rows, A).to(dt).to(DEV)
+    for dh, dn in ((d, None), (None, d)):
+        r, b = res.clone().requires_grad_(True), br.clone().requires_grad_(True)
+        hidden, normed = residual_block_norm(r, b, post, pre=pre)
+        out = hidden if dn is None else normed
+        params = [post.weight] + ([] if dn is None else [pre.weight, pre.bias])
+        got = torch.autograd.grad(out, [r, b] + params, d)
+        want = N.reference(res, br, None, _spec(post), _spec(pre), 1.0, 1.0, dh, dn)
+        for k, v in zip(("residual", "branch", "post_w", "pre_w", "pre_b"), got):
+            N.compare(k, v, want[k], dt)
+    hidden, normed = residual_block_norm(r, br, post, pre=pre)
+    hidden.backward(d)                                               # normed unused: the pre norm's parameters get zeros or nothing
+    assert pre.weight.grad is None or not bool(pre.weight.grad.any())
+    post.requires_grad_(False)
+    pre.requires_grad_(False)
+    r = res.clone().requires_grad_(True)
+    hidden, normed = residual_block_norm(r, br, post, pre=pre)
+    (gr,) = torch.autograd.grad([hidden, normed], [r], [d, d])
+    N.compare("residual", gr, N.reference(res, br, None, _spec(post), _spec(pre), 1.0, 1.0, d, d)["residual"], dt)
+
+
+def test_gradient_against_differences():
+    """<gradient, v> against central differences of the float64 forward along v."""
+    g = torch.Generator("cpu").manual_seed(14)
+    rows, A, dt = 6, 96, torch.float32
+    res, br, gate = _rand(g, rows, A).to(DEV), _rand(g, rows, A).to(DEV), _rand(g, rows, 1).to(DEV)
+    post, pre = _norm_module(g, A, "layer", dt), _norm_module(g, A, "rms", dt)
+    dh, dn = _rand(g, rows, A).to(DEV), _rand(g, rows, A).to(DEV)
+    leaves = [t.requires_grad_(True) for t in (res, br, gate)] + [post.weight, post.bias, pre.weight]
+    out = residual_block_norm(res, br, post, gate=gate, residual_scale=0.5, branch_scale=2.0, pre=pre)
+    grads = torch.autograd.grad(out, leaves, [dh, dn])
+    base = [t.detach().double() for t in leaves]
+
+    def loss(ts):
+        o = N.reference(ts[0], ts[1], ts[2], dict(_spec(post), w=ts[3], b=ts[4]), dict(_spec(pre), w=ts[5]), 0.5, 2.0)
+        return float((o["hidden"][0] * dh.double()).sum() + (o["normed"][0] * dn.double()).sum())
+
+    for i in range(len(leaves)):
+        v = _rand(g, *leaves[i].shape).double().to(DEV)
+        e = 1e-5
+        plus, minus = list(base), list(base)
+        plus[i], minus[i] = base[i] + e * v, base[i] - e * v
+        diff = (loss(plus) - loss(minus)) / (2 * e)
+        dot = float((grads[i].double() * v).sum())
+        # differences: e^2 third derivatives (~1e-9 of the terms) + float64 noise / e (~1e-10); gradient: fp32, K 2^-24 a term
+        scale = float((grads[i].double().abs() * v.abs()).sum())
+        assert abs(diff - dot) <= 2e-5 * scale, (i, diff, dot, scale)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_same_bits_twice_and_on_another_stream(dt):
+    g = torch.Generator("cpu").manual_seed(15)
+    rows, A = 3001, 768
+    res, br = _rand(g, rows, A).to(dt).to(DEV).requires_grad_(True), _rand(g, rows, A).to(dt).to(DEV).requires_grad_(True)
+    post, pre = _norm_module(g, A, "layer", dt), _norm_module(g, A, "layer", dt)
+    gate = _gate(g, "channel", rows, A, dt).requires_grad_(True)
+    d = _rand(g, rows, A).to(dt).to(DEV)
+    leaves = [res, br, gate] + list(post.parameters()) + list(pre.parameters())
+
+    def once():
+        out = residual_block_norm(res, br, post, gate=gate, pre=pre)
+        return list(out) + list(torch.autograd.grad(out, leaves, [d, d]))
+
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+def test_captured_and_replayed():
+    """Forward and backward recorded into one graph, replayed over new inputs with eager work in between."""
+    g = torch.Generator("cpu").manual_seed(16)
+    rows, A, dt = 65, 520, torch.bfloat16
+    post, pre = _norm_module(g, A, "rms", dt), _norm_module(g, A, "layer", dt)
+    leaves = [torch.zeros(rows, A, dtype=dt, device=DEV).requires_grad_(True) for _ in range(2)]
+    params = [post.weight, pre.weight, pre.bias]
+    d = _rand(g, rows, A).to(dt).to(DEV)
+
+    def step(res, br):
+        out = residual_block_norm(res, br, post, pre=pre)
+        return list(out) + list(torch.autograd.grad(out, [res, br] + params, [d, d]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*leaves)
+    for i in range(3):
+        x, y = _rand(g, rows, A).to(dt).to(DEV), _rand(g, rows, A).to(dt).to(DEV)
+        with torch.no_grad():
+            leaves[0].copy_(x)
+            leaves[1].copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(x.requires_grad_(True), y.requires_grad_(True))
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_c_call_leaves_gaps_and_later_rows_alone():
+    """Output rows at a larger stride: the columns between them and the rows behind the last stay as they were."""
+    from matryoshka_transcoder_amd.engine import _p, _stream
+    lib = _lib.load()
+    for A, ld in ((64, 80), (61, 67)):
+        rows = 5
+        x, y = torch.randn(rows, A, device=DEV), torch.randn(rows, A, device=DEV)
+        hidden, normed = torch.full((rows + 2, ld), 7.0, device=DEV), torch.full((rows + 2, ld), 7.0, device=DEV)
+        d = _lib.BlockNormDesc(rows=rows, A=A, dtype=_lib.MTC_F32, has_branch=1, pre_kind=_lib.MTC_NORM_RMS, pre_eps=1e-6,
+                               residual_scale=1.0, branch_scale=1.0, ld_residual=A, ld_branch=A, ld_hidden=ld, ld_normed=ld)
+        _lib.check(lib.mtc_block_norm_fwd(C.byref(d), _p(x), _p(y), None, None, None, None, None, _p(hidden), _p(normed), None,
+                                          _stream()))
+        torch.cuda.synchronize()
+        assert torch.equal(hidden[:rows, :A], x + y)
+        for o in (hidden, normed):
+            assert bool((o[rows:] == 7.0).all()) and bool((o[:, A:] == 7.0).all())
+
+
+def test_no_rows():
+    m = BlockNorm(64, kind="layer", dtype=torch.float32, device=DEV)
+    x = torch.zeros(0, 64, device=DEV, requires_grad=True)
+    y = torch.zeros(0, 64, device=DEV, requires_grad=True)
+    h, n = residual_block_norm(x, y, m, pre=m)
+    assert h.shape == n.shape == (0, 64)
+    (h.sum() + n.sum()).backward()
+    assert x.grad.shape == (0, 64) and not bool(m.weight.grad.any()) and not bool(m.bias.grad.any())
+    assert block_norm(torch.zeros(2, 0, 64, device=DEV)).shape == (2, 0, 64)
+
+
+def test_refusals_on_the_gpu():
+    x = torch.randn(4, 64, device=DEV)
+    with pytest.raises(_lib.MtcError, match="share shape"):
+        residual_block_norm(x, x.bfloat16())
+    with pytest.raises(_lib.MtcError, match="share shape"):
+        residual_block_norm(x, x[:3])
+    with pytest.raises(_lib.MtcError, match="width 32"):
+        residual_block_norm(x, x, BlockNorm(32, device=DEV))
+    with pytest.raises(_lib.MtcError, match="weight"):
+        block_norm(x, torch.ones(64, device=DEV, dtype=torch.bfloat16))
+    with pytest.raises(_lib.MtcError, match="weight"):
+        block_norm(x, torch.ones(64))
+    with pytest.raises(_lib.MtcError, match="gate of shape"):
+        residual_block_norm(x, x, gate=torch.ones(4, device=DEV))
+    with pytest.raises(_lib.MtcError, match="gate must be"):
+        residual_block_norm(x, x, gate=torch.ones(64))
+    with pytest.raises(_lib.MtcError, match="unsupported model dtype"):
+        block_norm(x.half())
+    with pytest.raises(_lib.MtcError, match="outside"):
+        block_norm(torch.zeros(1, 8200, device=DEV))
+    with pytest.raises(_lib.MtcError, match="at least one dimension"):
+        block_norm(torch.zeros((), device=DEV))
+    with pytest.raises(RuntimeError):                                # second derivatives are refused, not wrong
+        r = x.clone().requires_grad_(True)
+        (gr,) = torch.autograd.grad(block_norm(r).sum(), [r], create_graph=True)
+        gr.sum().backward()
