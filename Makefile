@@ -2,7 +2,7 @@
 HIPCC ?= /opt/rocm/bin/hipcc
 ARCH  ?= gfx950
 CSRC  := matryoshka_transcoder_amd/csrc
-SRCS  := $(CSRC)/api.hip $(CSRC)/encode.hip $(CSRC)/select.hip $(CSRC)/decode.hip $(CSRC)/backward.hip $(CSRC)/optim.hip $(CSRC)/aux.hip $(CSRC)/collect.hip $(CSRC)/store.hip $(CSRC)/comm.hip $(CSRC)/block_norm.hip
+SRCS  := $(CSRC)/api.hip $(CSRC)/encode.hip $(CSRC)/select.hip $(CSRC)/decode.hip $(CSRC)/backward.hip $(CSRC)/optim.hip $(CSRC)/aux.hip $(CSRC)/collect.hip $(CSRC)/store.hip $(CSRC)/comm.hip $(CSRC)/block_norm.hip $(CSRC)/grad_clip.hip
 OBJS  := $(SRCS:.hip=.o)
 LIB   := matryoshka_transcoder_amd/libmtc.so
 # no packed fp32 instructions: the compiler forms them from plain float code, and some of their forms are not reliable here

@@ -594,6 +594,32 @@ int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* residual, const
                        void* d_residual, void* d_branch, void* d_gate, void* d_post_w, void* d_post_b, void* d_pre_w,
                        void* d_pre_b, void* workspace, size_t workspace_bytes, void* stream);
 
+/* One norm over all gradients of a step and their scaling by it (the clipping cfg["max_grad_norm"] names, config.py:70; the
+ * reference's loop never performs it):
+ *     norm = (sum over all tensors of |g|^p)^(1/p), p = 1, 2 or infinity      coef = min(1, max_norm / (norm + 1e-6))
+ * n tensors given by HOST arrays: device pointers, element counts (0 = the tensor is skipped) and dtypes (MTC_F32 / MTC_BF16,
+ * mixed as they come).  Any alignment an element may have; 16-byte accesses where every address of a tensor allows them.
+ * Sums are held in 64 bits and added in a fixed order.  A NaN gives norm and coef NaN, an infinity coef 0 (NaN for
+ * max_norm = infinity).  workspace: mtc_grad_norm_workspace_bytes, 8-byte aligned, nothing in it needs clearing.
+ *   mtc_grad_norm      : *total = the sum before the root (optional; fp64, for adding up over ranks) and / or
+ *                        norm_coef[2] = {norm, coef} (optional)
+ *   mtc_grad_norm_coef : norm_coef[2] from such a total
+ *   mtc_grad_clip      : out[i] = round(grads[i] * coef), *norm_out = norm (optional).  out[i] = grads[i] clips in place, and
+ *                        then nothing is written when coef is 1.  Outputs that overlap anything else of the list are refused.
+ *   mtc_adam_flat_scaled, mtc_unitnorm_adam_rows_scaled : mtc_adam_flat / mtc_unitnorm_adam_rows on round(grad * *grad_scale)
+ *                        (device scalar: norm_coef + 1), bit for bit what clipping in place before them gives, without the pass. */
+size_t mtc_grad_norm_workspace_bytes(int32_t n, const uint64_t* elems_host, const int32_t* dtype_host);
+int mtc_grad_norm(int32_t n, const void* const* grads_host, const uint64_t* elems_host, const int32_t* dtype_host, float p,
+                  void* workspace, size_t workspace_bytes, double* total, float max_norm, float* norm_coef, void* stream);
+int mtc_grad_norm_coef(const double* total, float p, float max_norm, float* norm_coef, void* stream);
+int mtc_grad_clip(int32_t n, const void* const* grads_host, void* const* out_host, const uint64_t* elems_host,
+                  const int32_t* dtype_host, float p, float max_norm, void* workspace, size_t workspace_bytes,
+                  float* norm_out, void* stream);
+int mtc_adam_flat_scaled(int32_t dtype, size_t n, void* p, const void* grad, void* exp_avg, void* exp_avg_sq,
+                         const mtc_adam_hyper* h_host, const float* grad_scale, void* stream);
+int mtc_unitnorm_adam_rows_scaled(const mtc_desc* d, void* W_dec, void* grad, void* exp_avg, void* exp_avg_sq,
+                                  const mtc_adam_hyper* h_host, int write_grad, const float* grad_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

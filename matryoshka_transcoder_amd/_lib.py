@@ -129,6 +129,12 @@ PROTOTYPES = {
     "mtc_gather_row_pairs": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, P, P, P, P, P, P, P]),
     "mtc_collect_top_samples": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, P, P, P, P, P, C.c_float,
                                           C.c_int32, C.c_int32, P, P, P, P, P, P, P]),
+    "mtc_grad_norm_workspace_bytes": (C.c_size_t, [C.c_int32, P, P]),
+    "mtc_grad_norm": (C.c_int, [C.c_int32, P, P, P, C.c_float, P, C.c_size_t, P, C.c_float, P, P]),
+    "mtc_grad_norm_coef": (C.c_int, [P, C.c_float, C.c_float, P, P]),
+    "mtc_grad_clip": (C.c_int, [C.c_int32, P, P, P, P, C.c_float, C.c_float, P, C.c_size_t, P, P]),
+    "mtc_adam_flat_scaled": (C.c_int, [C.c_int32, C.c_size_t, P, P, P, P, HP, P, P]),
+    "mtc_unitnorm_adam_rows_scaled": (C.c_int, [DP, P, P, P, P, HP, C.c_int, P, P]),
     "mtc_block_norm_fwd": (C.c_int, [NP] + [P] * 11),
     "mtc_block_norm_bwd_workspace_bytes": (C.c_size_t, [NP]),
     "mtc_block_norm_bwd": (C.c_int, [NP] + [P] * 9 + [C.c_int64, P, C.c_int64] + [P] * 8 + [C.c_size_t, P]),

@@ -47,12 +47,27 @@ __device__ __forceinline__ void adam_elem(float& p, float g, float& m, float& v,
     p = D_::rnd(fmaf(k.neg_step, div_dt<DT>(m, den), p));
 }
 
-template <int DT>
+// the product rounded by itself: contracted into the Adam update's fma, an fp32 gradient would skip the rounding that a
+// scaled gradient in memory has
+template <int DT> __device__ __forceinline__ float scaled_grad(float g, float gs) {
+#pragma clang fp contract(off)
+    const float r = g * gs;
+    return DType<DT>::rnd(r);
+}
+
+// SCALED = 1: the gradient is multiplied by *grad_scale (the clipping coefficient) and rounded to the parameter dtype as it is
+// loaded, which is what a separate scaling pass would leave in memory -- without that pass.
+template <int DT, int SCALED>
 __global__ __launch_bounds__(256) void adam_flat_kernel(size_t n_chunks, void* __restrict__ p, const void* __restrict__ g,
-                                                        void* __restrict__ m, void* __restrict__ v, AdamK k) {
+                                                        void* __restrict__ m, void* __restrict__ v, AdamK k,
+                                                        const float* __restrict__ grad_scale) {
+    const float gs = SCALED ? *grad_scale : 1.f;
     for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < n_chunks; c += (size_t)gridDim.x * 256) {
         float pp[8], gg[8], mm[8], vv[8];
         load8<DT>(p, c * 8, pp); load8<DT>(g, c * 8, gg); load8<DT>(m, c * 8, mm); load8<DT>(v, c * 8, vv);
+        if (SCALED)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) gg[i] = scaled_grad<DT>(gg[i], gs);
 #pragma unroll
         for (int i = 0; i < 8; ++i) adam_elem<DT>(pp[i], gg[i], mm[i], vv[i], k);
         store8<DT>(p, c * 8, pp); store8<DT>(m, c * 8, mm); store8<DT>(v, c * 8, vv);
@@ -61,11 +76,13 @@ __global__ __launch_bounds__(256) void adam_flat_kernel(size_t n_chunks, void* _
 
 // wave per decoder row.  MODE 0: projection only (weights normalised, grad projected, written back)
 //                        MODE 1: projection + Adam (grad optionally written back)
+//                        MODE 2: the same on the gradient times *grad_scale, rounded (adam_flat_kernel's SCALED)
 template <int DT, int NC, int MODE>
 __global__ __launch_bounds__(256) void unitnorm_rows_kernel(int D, int A, void* __restrict__ W, void* __restrict__ grad,
                                                             void* __restrict__ m, void* __restrict__ v, AdamK k,
-                                                            int write_grad) {
+                                                            int write_grad, const float* __restrict__ grad_scale) {
     typedef DType<DT> D_;
+    const float gs = MODE == 2 ? *grad_scale : 1.f;
     const int lane = threadIdx.x & 63;
     const int j = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (j >= D) return;
@@ -78,6 +95,9 @@ __global__ __launch_bounds__(256) void unitnorm_rows_kernel(int D, int A, void* 
             const size_t off = (size_t)j * A + (size_t)(lane + 64 * c) * 8;
             load8<DT>(W, off, w[c]);
             load8<DT>(grad, off, g[c]);
+            if (MODE == 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[c][i] = scaled_grad<DT>(g[c][i], gs);
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(w[c][i], w[c][i], ss);
         }
@@ -102,7 +122,7 @@ __global__ __launch_bounds__(256) void unitnorm_rows_kernel(int D, int A, void* 
 #pragma unroll
             for (int i = 0; i < 8; ++i) g[c][i] = D_::rnd(g[c][i] - D_::rnd(dot * w[c][i]));
             if (MODE == 0 || write_grad) store8<DT>(grad, off, g[c]);
-            if (MODE == 1) {
+            if (MODE != 0) {
                 float mm[8], vv[8];
                 load8<DT>(m, off, mm); load8<DT>(v, off, vv);
 #pragma unroll
@@ -478,25 +498,42 @@ using namespace mtc;
     do {                                                                                                                     \
         const int nc_ = nc_for(d->A_t);                                                                                      \
         const dim3 grid((d->D + 3) / 4), block(256);                                                                         \
-        if (nc_ <= 1) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 1, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else if (nc_ <= 2) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 2, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else if (nc_ <= 3) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 3, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else if (nc_ <= 5) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 5, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else if (nc_ <= 7) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 7, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else if (nc_ <= 9) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 9, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
-        else hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 16, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad); \
+        if (nc_ <= 1) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 1, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else if (nc_ <= 2) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 2, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else if (nc_ <= 3) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 3, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else if (nc_ <= 5) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 5, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else if (nc_ <= 7) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 7, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else if (nc_ <= 9) hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 9, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
+        else hipLaunchKernelGGL((unitnorm_rows_kernel<DTV, 16, MODE>), grid, block, 0, s, d->D, d->A_t, W_dec, grad, m, v, k, write_grad, grad_scale); \
     } while (0)
+
+static int unitnorm_adam(const char* who, const mtc_desc* d, void* W_dec, void* grad, void* m, void* v,
+                         const mtc_adam_hyper* h_host, int write_grad, const float* grad_scale, void* stream) {
+    if (check_desc(d, who)) return -1;
+    MTC_REQUIRE(W_dec && grad && m && v && h_host, "%s: null pointer", who);
+    MTC_REQUIRE(h_host->step >= 1, "%s: step is 1-based", who);
+    const AdamK k = make_adam(h_host);
+    hipStream_t s = as_stream(stream);
+    if (grad_scale) {
+        if (d->dtype == MTC_BF16) LAUNCH_ROWS(MTC_BF16, 2);
+        else LAUNCH_ROWS(MTC_F32, 2);
+    } else {
+        if (d->dtype == MTC_BF16) LAUNCH_ROWS(MTC_BF16, 1);
+        else LAUNCH_ROWS(MTC_F32, 1);
+    }
+    return check_launch(who);
+}
 
 extern "C" int mtc_unitnorm_adam_rows(const mtc_desc* d, void* W_dec, void* grad, void* m, void* v,
                                       const mtc_adam_hyper* h_host, int write_grad, void* stream) {
-    if (check_desc(d, "mtc_unitnorm_adam_rows")) return -1;
-    MTC_REQUIRE(W_dec && grad && m && v && h_host, "mtc_unitnorm_adam_rows: null pointer");
-    MTC_REQUIRE(h_host->step >= 1, "mtc_unitnorm_adam_rows: step is 1-based");
-    const AdamK k = make_adam(h_host);
-    hipStream_t s = as_stream(stream);
-    if (d->dtype == MTC_BF16) LAUNCH_ROWS(MTC_BF16, 1);
-    else LAUNCH_ROWS(MTC_F32, 1);
-    return check_launch("mtc_unitnorm_adam_rows");
+    return unitnorm_adam("mtc_unitnorm_adam_rows", d, W_dec, grad, m, v, h_host, write_grad, nullptr, stream);
+}
+
+extern "C" int mtc_unitnorm_adam_rows_scaled(const mtc_desc* d, void* W_dec, void* grad, void* m, void* v,
+                                             const mtc_adam_hyper* h_host, int write_grad, const float* grad_scale,
+                                             void* stream) {
+    MTC_REQUIRE(grad_scale, "mtc_unitnorm_adam_rows_scaled: null grad_scale");
+    return unitnorm_adam("mtc_unitnorm_adam_rows_scaled", d, W_dec, grad, m, v, h_host, write_grad, grad_scale, stream);
 }
 
 extern "C" int mtc_unitnorm_project(const mtc_desc* d, void* W_dec, void* grad, void* stream) {
@@ -505,6 +542,7 @@ extern "C" int mtc_unitnorm_project(const mtc_desc* d, void* W_dec, void* grad, 
     AdamK k = {};
     void* m = nullptr; void* v = nullptr;
     const int write_grad = 1;
+    const float* grad_scale = nullptr;
     hipStream_t s = as_stream(stream);
     if (d->dtype == MTC_BF16) LAUNCH_ROWS(MTC_BF16, 0);
     else LAUNCH_ROWS(MTC_F32, 0);
@@ -549,21 +587,36 @@ extern "C" int mtc_fused_set_sliced(int mode) {
     return prev;
 }
 
-extern "C" int mtc_adam_flat(int32_t dtype, size_t n, void* p, const void* grad, void* m, void* v,
-                             const mtc_adam_hyper* h_host, void* stream) {
-    MTC_REQUIRE(p && grad && m && v && h_host, "mtc_adam_flat: null pointer");
-    MTC_REQUIRE((n & 7) == 0, "mtc_adam_flat: element count must be a multiple of 8 (got %zu)", n);
-    MTC_REQUIRE(dtype == MTC_F32 || dtype == MTC_BF16, "mtc_adam_flat: bad dtype");
-    MTC_REQUIRE(h_host->step >= 1, "mtc_adam_flat: step is 1-based");
+static int adam_flat(const char* who, int32_t dtype, size_t n, void* p, const void* grad, void* m, void* v,
+                     const mtc_adam_hyper* h_host, const float* grad_scale, void* stream) {
+    MTC_REQUIRE(p && grad && m && v && h_host, "%s: null pointer", who);
+    MTC_REQUIRE((n & 7) == 0, "%s: element count must be a multiple of 8 (got %zu)", who, n);
+    MTC_REQUIRE(dtype == MTC_F32 || dtype == MTC_BF16, "%s: bad dtype", who);
+    MTC_REQUIRE(h_host->step >= 1, "%s: step is 1-based", who);
     if (n == 0) return 0;
     const AdamK k = make_adam(h_host);
     const size_t n_chunks = n / 8;
-    const int grid = (int)std::min<size_t>((n_chunks + 255) / 256, 4096);
-    if (dtype == MTC_BF16)
-        hipLaunchKernelGGL(adam_flat_kernel<MTC_BF16>, dim3(grid), dim3(256), 0, as_stream(stream), n_chunks, p, grad, m, v, k);
-    else
-        hipLaunchKernelGGL(adam_flat_kernel<MTC_F32>, dim3(grid), dim3(256), 0, as_stream(stream), n_chunks, p, grad, m, v, k);
-    return check_launch("mtc_adam_flat");
+    const dim3 grid((unsigned)std::min<size_t>((n_chunks + 255) / 256, 4096)), block(256);
+    hipStream_t s = as_stream(stream);
+    if (dtype == MTC_BF16) {
+        if (grad_scale) hipLaunchKernelGGL((adam_flat_kernel<MTC_BF16, 1>), grid, block, 0, s, n_chunks, p, grad, m, v, k, grad_scale);
+        else hipLaunchKernelGGL((adam_flat_kernel<MTC_BF16, 0>), grid, block, 0, s, n_chunks, p, grad, m, v, k, grad_scale);
+    } else {
+        if (grad_scale) hipLaunchKernelGGL((adam_flat_kernel<MTC_F32, 1>), grid, block, 0, s, n_chunks, p, grad, m, v, k, grad_scale);
+        else hipLaunchKernelGGL((adam_flat_kernel<MTC_F32, 0>), grid, block, 0, s, n_chunks, p, grad, m, v, k, grad_scale);
+    }
+    return check_launch(who);
+}
+
+extern "C" int mtc_adam_flat(int32_t dtype, size_t n, void* p, const void* grad, void* m, void* v,
+                             const mtc_adam_hyper* h_host, void* stream) {
+    return adam_flat("mtc_adam_flat", dtype, n, p, grad, m, v, h_host, nullptr, stream);
+}
+
+extern "C" int mtc_adam_flat_scaled(int32_t dtype, size_t n, void* p, const void* grad, void* m, void* v,
+                                    const mtc_adam_hyper* h_host, const float* grad_scale, void* stream) {
+    MTC_REQUIRE(grad_scale, "mtc_adam_flat_scaled: null grad_scale");
+    return adam_flat("mtc_adam_flat_scaled", dtype, n, p, grad, m, v, h_host, grad_scale, stream);
 }
 
 #define LAUNCH_FUSED_NC(DTV, COEF, PROJ, DOT, EX, NCV)                                                                          \

@@ -526,16 +526,25 @@ class HotPath:
         d = self.desc(1)
         check(self.lib.mtc_unitnorm_project(C.byref(d), _p(W_dec), _p(grad), _stream()), "mtc_unitnorm_project")
 
-    def unitnorm_adam(self, W_dec, grad, m, v, hyper: AdamHyper, write_grad: bool = True):
+    def unitnorm_adam(self, W_dec, grad, m, v, hyper: AdamHyper, write_grad: bool = True, grad_scale=None):
+        """grad_scale: device pointer of the clipping coefficient the gradient is multiplied by as it is read (None = 1)."""
         for t, n in ((W_dec, "W_dec"), (grad, "W_dec.grad"), (m, "exp_avg"), (v, "exp_avg_sq")):
             _need(t, n, self.dtype, (self.D, self.A_t))
         d = self.desc(1)
+        if grad_scale is not None:
+            check(self.lib.mtc_unitnorm_adam_rows_scaled(C.byref(d), _p(W_dec), _p(grad), _p(m), _p(v), C.byref(hyper),
+                                                         int(write_grad), grad_scale, _stream()), "mtc_unitnorm_adam_rows_scaled")
+            return
         check(self.lib.mtc_unitnorm_adam_rows(C.byref(d), _p(W_dec), _p(grad), _p(m), _p(v), C.byref(hyper),
                                               int(write_grad), _stream()), "mtc_unitnorm_adam_rows")
 
-    def adam_flat(self, p, grad, m, v, hyper: AdamHyper):
+    def adam_flat(self, p, grad, m, v, hyper: AdamHyper, grad_scale=None):
         for t, n in ((p, "param"), (grad, "grad"), (m, "exp_avg"), (v, "exp_avg_sq")):
             _need(t, n, self.dtype)
+        if grad_scale is not None:
+            check(self.lib.mtc_adam_flat_scaled(self.code, p.numel(), _p(p), _p(grad), _p(m), _p(v), C.byref(hyper), grad_scale,
+                                                _stream()), "mtc_adam_flat_scaled")
+            return
         check(self.lib.mtc_adam_flat(self.code, p.numel(), _p(p), _p(grad), _p(m), _p(v), C.byref(hyper), _stream()),
               "mtc_adam_flat")
 

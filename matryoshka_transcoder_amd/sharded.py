@@ -32,6 +32,7 @@ import torch.distributed as dist
 
 from . import _lib
 from .engine import HotPath, Selection, _p, _stream, check
+from .grad_clip import coef_of_power_sum, power_sum
 from .training import FusedAdam
 from .transcoder import MatryoshkaTranscoder, _feature_major
 
@@ -735,4 +736,17 @@ class ShardedMatryoshkaTranscoder(MatryoshkaTranscoder):
 
 
 class ShardedFusedAdam(FusedAdam):
-    """FusedAdam over the local shard; nothing to exchange (b_dec's gradient is identical on all ranks)."""
+    """FusedAdam over the local shard; nothing to exchange (b_dec's gradient is identical on all ranks), but with
+    max_grad_norm the norm is the whole dictionary's: the shards' sums of squares, fp64, are gathered and added in rank order
+    (the same coefficient, bit for bit, on every rank), b_dec's counts once."""
+
+    def _norm_and_coef(self, params):
+        tc = self.transcoder
+        local, shared = [p.grad for p in params if p is not tc.b_dec], [p.grad for p in params if p is tc.b_dec]
+        total = torch.zeros((), dtype=torch.float64, device=params[0].device)
+        if local:
+            mine = power_sum(local).reshape(1).view(torch.int64)         # 8 bytes as they are: libmtc's transport has no fp64
+            total = total + tc.comm.all_gather(mine, tag="grad norm").view(torch.float64).sum()
+        if shared:
+            total = total + power_sum(shared)
+        return coef_of_power_sum(total, self.max_grad_norm)

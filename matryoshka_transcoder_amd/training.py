@@ -16,7 +16,8 @@ import torch
 
 from . import _lib
 from .activation_samples import ActivationSampleCollector
-from .engine import adam_hyper
+from .engine import _p, adam_hyper
+from .grad_clip import norm_and_coef
 from .results import CleanResultsManager
 
 
@@ -53,10 +54,19 @@ class FusedAdam(torch.optim.Optimizer):
     """torch.optim.Adam semantics (eps 1e-8, no weight decay / amsgrad; moments in the parameter
     dtype) executed by libmtc.  `step()` assumes the caller already ran
     `transcoder.make_decoder_weights_and_grad_unit_norm()` like the reference loop does;
-    `step(project=True)` fuses that projection into the W_dec update (one pass over W_dec)."""
+    `step(project=True)` fuses that projection into the W_dec update (one pass over W_dec).
 
-    def __init__(self, transcoder, lr=3e-4, betas=(0.9, 0.99), eps=1e-8):
+    max_grad_norm: clip the gradients' common 2-norm to it (grad_clip.py) before the projection and the update; the
+    coefficient is applied as the gradients are read, with the bits that clipping them in place first would give, and the
+    `.grad` tensors stay as they are.  `last_grad_norm` then holds the norm before clipping (float32 scalar on the GPU).
+    `train_step` materialises the gradients in that case: their norm has to be known before the first parameter moves."""
+
+    def __init__(self, transcoder, lr=3e-4, betas=(0.9, 0.99), eps=1e-8, max_grad_norm: Optional[float] = None):
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise _lib.MtcError(f"max_grad_norm must not be negative or NaN, got {max_grad_norm}")
         self.transcoder = transcoder
+        self.max_grad_norm = max_grad_norm
+        self.last_grad_norm = None
         super().__init__(list(transcoder.parameters()), dict(lr=lr, betas=betas, eps=eps))
 
     def _state(self, p):
@@ -82,6 +92,10 @@ class FusedAdam(torch.optim.Optimizer):
 
     def _train_step(self, x_source, x_target):
         tc = self.transcoder
+        if self.max_grad_norm is not None:
+            res = tc._run_forward(x_source, x_target, tc.W_enc, tc.b_enc, tc.W_dec, tc.b_dec, True)
+            tc._last_res = res
+            return self._dense_step(res, x_target)
         tc._defer_dvals = True          # d a_bj comes out of the decoder-gradient kernel below
         if getattr(tc, "_side_stream", None) is None and getattr(tc, "_overlap_ok", True) and x_source.is_cuda:
             tc._side_stream = torch.cuda.Stream(device=x_source.device)
@@ -101,11 +115,7 @@ class FusedAdam(torch.optim.Optimizer):
             tc._join_csc()
             if two_streams:
                 torch.cuda.current_stream().wait_stream(tc._side_stream)
-            dW_dec, dW_encT, db_enc, db_dec = tc._run_backward(res, None)
-            tc.W_dec.grad, tc.W_enc.grad, tc.b_enc.grad, tc.b_dec.grad = dW_dec, dW_encT.t(), db_enc, db_dec
-            self.step(project=True)
-            self.zero_grad()
-            return tc._output_dict(res, x_target)
+            return self._dense_step(res, x_target)
         group = self.param_groups[0]
         b1, b2 = group["betas"]
         hy = {}
@@ -146,6 +156,19 @@ class FusedAdam(torch.optim.Optimizer):
             update_b_dec()
         return tc._output_dict(res, x_target)               # (flushes what the forward chain deferred behind the backward launches)
 
+    def _dense_step(self, res, x_target):
+        """The step's second half with the four gradients in memory."""
+        tc = self.transcoder
+        dW_dec, dW_encT, db_enc, db_dec = tc._run_backward(res, None)
+        tc.W_dec.grad, tc.W_enc.grad, tc.b_enc.grad, tc.b_dec.grad = dW_dec, dW_encT.t(), db_enc, db_dec
+        self.step(project=True)
+        self.zero_grad()
+        return tc._output_dict(res, x_target)
+
+    def _norm_and_coef(self, params):
+        """{norm, clipping coefficient} of the parameters' gradients.  Overridden by the feature-sharded optimizer."""
+        return norm_and_coef([p.grad for p in params], self.max_grad_norm)
+
     @torch.no_grad()
     def step(self, closure=None, project: bool = False):
         if closure is not None:
@@ -156,6 +179,12 @@ class FusedAdam(torch.optim.Optimizer):
     def _step(self, project: bool):
         tc = self.transcoder
         hp = tc.hot_path()
+        scale = None
+        if self.max_grad_norm is not None:
+            live = [p for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if live:
+                nc = self._norm_and_coef(live)
+                self.last_grad_norm, scale = nc[0], _p(nc[1:])
         for group in self.param_groups:
             b1, b2 = group["betas"]
             for p in group["params"]:
@@ -166,7 +195,7 @@ class FusedAdam(torch.optim.Optimizer):
                 h = adam_hyper(group["lr"], b1, b2, group["eps"], st["step"])
                 if p is tc.W_dec and project:
                     g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-                    hp.unitnorm_adam(p.data, g, st["exp_avg"], st["exp_avg_sq"], h, write_grad=False)
+                    hp.unitnorm_adam(p.data, g, st["exp_avg"], st["exp_avg_sq"], h, write_grad=False, grad_scale=scale)
                 elif p is tc.W_enc:
                     # feature-major storage: run on the contiguous transposed views
                     tc._w_encT(p)
@@ -176,19 +205,21 @@ class FusedAdam(torch.optim.Optimizer):
                     if not m.is_contiguous():
                         st["exp_avg"] = m.contiguous().t(); st["exp_avg_sq"] = v.contiguous().t()
                         m, v = st["exp_avg"].t(), st["exp_avg_sq"].t()
-                    hp.adam_flat(p.data.t(), g, m, v, h)
+                    hp.adam_flat(p.data.t(), g, m, v, h, grad_scale=scale)
                 else:
                     g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-                    hp.adam_flat(p.data, g, st["exp_avg"], st["exp_avg_sq"], h)
+                    hp.adam_flat(p.data, g, st["exp_avg"], st["exp_avg_sq"], h, grad_scale=scale)
         return None
 
 
 # ------------------------------------------------------------------ the loop (training.py:49-213)
 def train_transcoder(transcoder, activation_store, model, cfg):
     """Train one transcoder.  `activation_store` is anything with `next_batch() -> (source, target)` on
-    cfg["device"] in cfg["dtype"]; `model` (the language model) is only handed through."""
+    cfg["device"] in cfg["dtype"]; `model` (the language model) is only handed through.  cfg["clip_gradients"] = True (not
+    in the reference, which never clips) applies cfg["max_grad_norm"] and logs the norm."""
     num_batches = int(cfg["num_tokens"] // cfg["batch_size"])
-    optimizer = FusedAdam(transcoder, lr=cfg["lr"], betas=(cfg["beta1"], cfg["beta2"]))
+    optimizer = FusedAdam(transcoder, lr=cfg["lr"], betas=(cfg["beta1"], cfg["beta2"]),
+                          max_grad_norm=cfg["max_grad_norm"] if cfg.get("clip_gradients", False) else None)
     scheduler = create_scheduler(optimizer, cfg, num_batches)
     results = CleanResultsManager(cfg.get("results_root", "results"))
     exp_dir = results.create_experiment_dir(cfg.get("model_name", "model"), cfg.get("layer", 0), num_batches,
@@ -235,6 +266,8 @@ def train_transcoder(transcoder, activation_store, model, cfg):
                 rec = metrics_of(out)
                 rec.update(step=i, dead_features_count=int((transcoder.num_batches_not_active >= n_dead_at).sum()),
                            learning_rate=optimizer.param_groups[0]["lr"], elapsed_s=time.time() - t0)
+                if optimizer.last_grad_norm is not None:
+                    rec["grad_norm"] = float(optimizer.last_grad_norm)
                 log.write(json.dumps(rec) + "\n")
             if scheduler is not None:
                 scheduler.step()
