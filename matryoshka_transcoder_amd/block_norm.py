@@ -214,7 +214,7 @@ class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, p, *tensors):
         residual = tensors[0]
-        stats = torch.empty(4, residual.numel() // p.A, dtype=torch.float32, device=residual.device)
+        stats = torch.empty(residual.numel() // p.A, 4, dtype=torch.float32, device=residual.device)
         hidden, normed = _forward(p, tensors, stats)
         ctx.plan = p
         ctx.set_materialize_grads(False)

@@ -14,6 +14,7 @@
 // workgroup holds `groups` such row groups.  Row sums: DPP inside a wave, one LDS exchange across the row's waves.
 // Rows whose width is a multiple of 8 with 16-byte-aligned rows use 16-byte accesses (columns 8 t .. 8 t + 7); any other
 // width or stride takes the same kernel with single elements (columns t, t + T, ..., which keeps a wave's accesses side by side).
+#include <type_traits>
 #include "common.hpp"
 
 namespace mtc {
@@ -33,10 +34,9 @@ struct NormArgs {
     float post_eps, pre_eps, post_off, pre_off, res_scale, branch_scale, inv_A;
     NormRow residual, branch, gate, hidden, normed;
     const void *post_w, *post_b, *pre_w, *pre_b;
-    float* stats;                        // [4][rows]: post mean, post rstd, pre mean, pre rstd
+    float* stats;                        // [rows][4]: post mean, post rstd, pre mean, pre rstd
     // backward
-    NormRow d_hidden, d_normed;
-    void *d_residual, *d_branch, *d_gate;
+    NormRow d_hidden, d_normed, d_residual, d_branch, d_gate;
     float* partial;                      // [workgroup][4 vectors of `pitch` floats, then the scalar gate's sum]
     int pitch, want_x1, want_x2, want_x3, want_x4, want_scalar;
 };
@@ -80,52 +80,94 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* sm, int& slot, i
     for (int n = 0; n < N; ++n) v[n] = lane_value(row16_sum_at15(lane < waves ? s[(lane & 15) * 4 + n] : 0.f), 15);
 }
 
-// the 8 columns of thread t
-template <int DT, bool VEC> struct Cols {
+// Rows are read and written through buffer instructions: a descriptor per row (built in scalar registers) whose size is the
+// row's, so that threads beyond the width read zeros and write nothing WITHOUT a branch.  Branches around the memory
+// instructions made the compiler wait for every load in flight at each join, which undid the prefetch below (a row's
+// loads then cost their full latency: 16384 x 4608 bf16, pair: forward 148 instead of 118 us, backward 329 instead of 178).
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t rows_rsrc(const void* base, long long byte_off, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + byte_off, 0, bytes, 0x00020000);
+}
+
+// the 8 columns of thread t, and 8 values as they lie in memory: what a load in flight occupies
+//   STREAM: non-temporal accesses, for passes over more than the Infinity Cache holds
+template <int DT, bool VEC, bool STREAM> struct Cols {
+    static constexpr int AUX = STREAM ? 2 : 0;
+    typedef typename DType<DT>::T T_;
+    static constexpr int ES = (int)sizeof(T_);
+    static constexpr int NR = VEC ? 8 * ES / 16 : 8;
+    struct Raw {
+        typedef std::conditional_t<VEC, u32x4, T_> R;
+        R r[NR];
+        __device__ __forceinline__ void unpack(float (&v)[8]) const {
+            if constexpr (VEC && DT == MTC_BF16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = __uint_as_float(r[0][i] << 16);
+                    v[2 * i + 1] = __uint_as_float(r[0][i] & 0xffff0000u);
+                }
+            } else if constexpr (VEC) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i >> 2][i & 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = DType<DT>::ld(&r[i]);
+            }
+        }
+    };
     int t, T, A;
-    __device__ __forceinline__ int col(int i) const { return VEC ? t * 8 + i : t + T * i; }
-    __device__ __forceinline__ bool in(int i) const { return VEC ? t * 8 < A : t + T * i < A; }
-    // elements outside the row read as zero
-    __device__ __forceinline__ void load(const void* base, long long off, float (&v)[8]) const {
-        typedef typename DType<DT>::T T_;
-        if (VEC) {
-            if (in(0)) load8<DT>(base, (size_t)(off + t * 8), v);
-            else
+    // bf16: 8 columns in a row; fp32: two runs of 4, T quads apart, so that every 16-byte access of a wave is contiguous
+    __device__ __forceinline__ int col(int i) const {
+        return !VEC ? t + T * i : ES == 2 ? t * 8 + i : (i < 4 ? t * 4 + i : (T + t) * 4 + i - 4);
+    }
+    __device__ __forceinline__ bool in(int i) const { return col(VEC ? i & ~(16 / ES - 1) : i) < A; }
+    __device__ __forceinline__ void fetch(rsrc_t s, Raw& q) const {
+        if constexpr (VEC) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.f;
+            for (int i = 0; i < NR; ++i) q.r[i] = __builtin_amdgcn_raw_buffer_load_b128(s, col(i * (16 / ES)) * ES, 0, AUX);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = in(i) ? DType<DT>::ld(reinterpret_cast<const T_*>(base) + off + col(i)) : 0.f;
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (ES == 2) q.r[i] = __builtin_amdgcn_raw_buffer_load_b16(s, col(i) * ES, 0, 0);
+                else q.r[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(s, col(i) * ES, 0, 0));
+            }
         }
     }
-    __device__ __forceinline__ void store(void* base, long long off, const float (&v)[8]) const {
-        typedef typename DType<DT>::T T_;
-        if (VEC) {
-            if (in(0)) store8<DT>(base, (size_t)(off + t * 8), v);
+    // `present` = false: zeros, and nothing is read
+    __device__ __forceinline__ void fetch(const NormRow& o, long long row, bool present, Raw& q) const {
+        fetch(rows_rsrc(o.p, row * o.ld * ES, present ? A * ES : 0), q);
+    }
+    __device__ __forceinline__ void store(rsrc_t s, const float (&v)[8]) const {
+        if constexpr (VEC && DT == MTC_BF16) {
+            u32x4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+            __builtin_amdgcn_raw_buffer_store_b128(r, s, t * 8 * ES, 0, AUX);
+        } else if constexpr (VEC) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                u32x4 r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[4 * k + i]);
+                __builtin_amdgcn_raw_buffer_store_b128(r, s, col(4 * k) * ES, 0, AUX);
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (in(i)) DType<DT>::st(reinterpret_cast<T_*>(base) + off + col(i), v[i]);
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (ES == 2) __builtin_amdgcn_raw_buffer_store_b16((u16)f32_to_bf16_bits(v[i]), s, col(i) * ES, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i]), s, col(i) * ES, 0, 0);
+            }
         }
     }
-    // offset + w, or 1 without a weight; 0 outside the row
-    __device__ __forceinline__ void weight(const void* w, float offset, float (&v)[8]) const {
-        if (w) load(w, 0, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = in(i) ? (w ? offset + v[i] : 1.f) : 0.f;
-    }
-    __device__ __forceinline__ void bias(const void* b, float (&v)[8]) const {
-        if (b) load(b, 0, v);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    __device__ __forceinline__ void store(const NormRow& o, long long row, bool present, const float (&v)[8]) const {
+        store(rows_rsrc(o.p, row * o.ld * ES, present ? A * ES : 0), v);
     }
 };
 
 // mean and 1/std of a row held in registers: v becomes u.  The variance is summed over v - mu (not as E[x^2] - mu^2,
 // which cancels for rows far from zero).
-template <int DT, bool VEC>
-__device__ __forceinline__ void normalise(const Cols<DT, VEC>& c, int kind, float eps, float inv_A, float (&v)[8], float* sm,
+template <typename COLS>
+__device__ __forceinline__ void normalise(const COLS& c, int kind, float eps, float inv_A, float (&v)[8], float* sm,
                                           int& slot, int group, int waves, float& mu, float& rstd) {
     mu = 0.f;
     if (kind == MTC_NORM_LAYER) {
@@ -146,63 +188,130 @@ __device__ __forceinline__ void normalise(const Cols<DT, VEC>& c, int kind, floa
     for (int i = 0; i < 8; ++i) v[i] *= rstd;
 }
 
-// factor and bias of the branch before the row / element gate: z = u_p * pf + pb
-template <int DT, bool VEC>
-__device__ __forceinline__ void branch_factors(const Cols<DT, VEC>& c, const NormArgs& a, float (&pf)[8], float (&pb)[8]) {
-    c.weight(a.post_kind == MTC_NORM_NONE ? nullptr : a.post_w, a.post_off, pf);
-    c.bias(a.post_kind == MTC_NORM_NONE ? nullptr : a.post_b, pb);
-    float cg[8];
-    if (a.gate_kind == MTC_GATE_CHANNEL) c.load(a.gate.p, 0, cg);
+// The weights a thread keeps for the launch: the branch before the row / element gate is z = u_p * pf + pb, the pre norm
+// u * qw + qb.  All loads go out before the first is waited for; an absent operand reads as zeros.
+struct NormWeights {
+    float pf[8], pb[8], qw[8], qb[8];
+    template <typename COLS> __device__ __forceinline__ void load(const COLS& c, const NormArgs& a, bool branch, bool pre) {
+        typename COLS::Raw w0, b0, g0, w1, b1;
+        const bool post = branch && a.post_kind != MTC_NORM_NONE, chan = branch && a.gate_kind == MTC_GATE_CHANNEL;
+        const bool pw = post && a.post_w, qw_ = pre && a.pre_w;
+        if (branch) {
+            c.fetch(NormRow{const_cast<void*>(a.post_w), 0}, 0, pw, w0);
+            c.fetch(NormRow{const_cast<void*>(a.post_b), 0}, 0, post && a.post_b, b0);
+            c.fetch(NormRow{a.gate.p, 0}, 0, chan, g0);
+        }
+        if (pre) {
+            c.fetch(NormRow{const_cast<void*>(a.pre_w), 0}, 0, qw_, w1);
+            c.fetch(NormRow{const_cast<void*>(a.pre_b), 0}, 0, a.pre_b != nullptr, b1);
+        }
+        if (branch) {
+            float g[8];
+            w0.unpack(pf);
+            b0.unpack(pb);
+            g0.unpack(g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float s = a.gate_kind == MTC_GATE_CHANNEL ? a.branch_scale * cg[i] : a.branch_scale;
-        pf[i] *= s;
-        pb[i] *= s;
+            for (int i = 0; i < 8; ++i) {
+                const float s = c.in(i) ? (chan ? a.branch_scale * g[i] : a.branch_scale) : 0.f;
+                pf[i] = s * (pw ? a.post_off + pf[i] : 1.f);
+                pb[i] *= s;
+            }
+        }
+        if (pre) {
+            w1.unpack(qw);
+            b1.unpack(qb);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qw[i] = c.in(i) ? (qw_ ? a.pre_off + qw[i] : 1.f) : 0.f;
+        }
+    }
+};
+
+// Walks a group's rows, two sets of operands in turn: while one row is computed, the next one's loads are in flight (the
+// two sets have names of their own: moving a register that a load has yet to fill would wait for it).
+template <bool PREFETCH, typename ROW, typename FETCH, typename COMPUTE>
+__device__ __forceinline__ void walk_rows(long long base, long long step, long long rows, FETCH fetch, ROW& s0, COMPUTE compute) {
+    if constexpr (!PREFETCH) {
+        for (; base < rows; base += step) {
+            compute(base, s0);
+            if (base + step < rows) fetch(base + step, s0);
+        }
+    } else {
+        ROW s1;
+        while (base < rows) {
+            fetch(base + step, s1);
+            compute(base, s0);
+            base += step;
+            if (base >= rows) break;
+            fetch(base + step, s0);
+            compute(base, s1);
+            base += step;
+        }
     }
 }
 
-template <int DT, bool VEC, bool BRANCH, bool PRE>
+template <typename COLS, bool FULL> struct FwdRow {
+    typename COLS::Raw residual, branch, gate[FULL ? 1 : 0];
+    uint32_t gr;                         // the row's gate as it lies in memory
+};
+
+template <int DT> __device__ __forceinline__ uint32_t fetch_one(const NormRow& o, long long row, bool present) {
+    constexpr int ES = (int)sizeof(typename DType<DT>::T);
+    const rsrc_t s = rows_rsrc(o.p, row * o.ld * ES, present ? ES : 0);
+    if constexpr (ES == 2) return (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(s, 0, 0, 0) << 16;
+    else return __builtin_amdgcn_raw_buffer_load_b32(s, 0, 0, 0);
+}
+
+template <int DT, bool VEC, bool BRANCH, bool PRE, bool FULL, bool STREAM>
 __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
-    typedef typename DType<DT>::T T_;
     __shared__ float sm[2 * 16 * 4];
     const int waves = a.T >> 6;
     const int group = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) / waves);
-    const Cols<DT, VEC> c = {(int)threadIdx.x - group * a.T, a.T, a.A};
+    const Cols<DT, VEC, STREAM> c = {(int)threadIdx.x - group * a.T, a.T, a.A};
     int slot = 0;
-    float pf[8], pb[8], qw[8], qb[8];
-    if (BRANCH) branch_factors(c, a, pf, pb);
-    if (PRE) { c.weight(a.pre_w, a.pre_off, qw); c.bias(a.pre_b, qb); }
-    for (long long base = (long long)blockIdx.x * a.groups; base < a.rows; base += (long long)gridDim.x * a.groups) {
+    const bool row_gate = a.gate_kind == MTC_GATE_ROW || a.gate_kind == MTC_GATE_SCALAR;         // scalar: ld = 0
+    const long long base0 = (long long)blockIdx.x * a.groups, step = (long long)gridDim.x * a.groups;
+    typedef FwdRow<Cols<DT, VEC, STREAM>, FULL> Row;
+    auto fetch = [&](long long base, Row& q) {
         const bool live = base + group < a.rows;
-        const long long row = live ? base + group : a.rows - 1;       // groups behind the last row repeat it and store nothing
-        float h[8];
-        c.load(a.residual.p, row * a.residual.ld, h);
+        const long long row = live ? base + group : 0;
+        c.fetch(a.residual, row, live, q.residual);
         if (BRANCH) {
-            float y[8], g[8], gr = 1.f, mu = 0.f, rstd = 1.f;
-            c.load(a.branch.p, row * a.branch.ld, y);
-            if (a.gate_kind == MTC_GATE_FULL) c.load(a.gate.p, row * a.gate.ld, g);
-            if (a.gate_kind == MTC_GATE_ROW || a.gate_kind == MTC_GATE_SCALAR)
-                gr = DType<DT>::ld(reinterpret_cast<const T_*>(a.gate.p) + row * a.gate.ld);       // scalar: ld = 0
-            if (a.post_kind != MTC_NORM_NONE) {
-                normalise(c, a.post_kind, a.post_eps, a.inv_A, y, sm, slot, group, waves, mu, rstd);
-                if (a.stats && live && c.t == 0) { a.stats[row] = mu; a.stats[a.rows + row] = rstd; }
-            }
+            c.fetch(a.branch, row, live, q.branch);
+            if (FULL) c.fetch(a.gate, row, live, q.gate[0]);
+            else q.gr = fetch_one<DT>(a.gate, row, live && row_gate);
+        }
+    };
+    Row first;
+    fetch(base0, first);
+    NormWeights w;
+    w.load(c, a, BRANCH, PRE);
+    walk_rows<VEC>(base0, step, a.rows, fetch, first, [&](long long base, const Row& q) {
+        const bool live = base + group < a.rows;                  // groups behind the last row compute on zeros and store nothing
+        const long long row = live ? base + group : 0;
+        float h[8], st[4] = {0.f, 0.f, 0.f, 0.f};
+        q.residual.unpack(h);
+        if (BRANCH) {
+            float y[8], g[8];
+            q.branch.unpack(y);
+            if (FULL) q.gate[0].unpack(g);
+            const float gr = row_gate ? __uint_as_float(q.gr) : 1.f;
+            if (a.post_kind != MTC_NORM_NONE)
+                normalise(c, a.post_kind, a.post_eps, a.inv_A, y, sm, slot, group, waves, st[0], st[1]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float z = fmaf(y[i], pf[i], pb[i]);
-                h[i] = fmaf(a.gate_kind == MTC_GATE_FULL ? g[i] : gr, z, a.res_scale * h[i]);
-            }
-            if (live) c.store(a.hidden.p, row * a.hidden.ld, h);
+            for (int i = 0; i < 8; ++i) h[i] = fmaf(FULL ? g[i] : gr, fmaf(y[i], w.pf[i], w.pb[i]), a.res_scale * h[i]);
+            c.store(a.hidden, row, live, h);
         }
         if (PRE) {
-            float mu, rstd;
-            normalise(c, a.pre_kind, a.pre_eps, a.inv_A, h, sm, slot, group, waves, mu, rstd);
-            if (a.stats && live && c.t == 0) { a.stats[2 * a.rows + row] = mu; a.stats[3 * a.rows + row] = rstd; }
+            normalise(c, a.pre_kind, a.pre_eps, a.inv_A, h, sm, slot, group, waves, st[2], st[3]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = fmaf(h[i], qw[i], qb[i]);
-            if (live) c.store(a.normed.p, row * a.normed.ld, h);
+            for (int i = 0; i < 8; ++i) h[i] = fmaf(h[i], w.qw[i], w.qb[i]);
+            c.store(a.normed, row, live, h);
         }
-    }
+        if (a.stats && c.t == 0) {
+            const u32x4 v = {__float_as_uint(st[0]), __float_as_uint(st[1]), __float_as_uint(st[2]), __float_as_uint(st[3])};
+            __builtin_amdgcn_raw_buffer_store_b128(v, rows_rsrc(a.stats, row * 16, live ? 16 : 0), 0, 0, 0);
+        }
+    });
 }
 
 // Gradient.  With g = d_normed, du = g (offset + w_pre):
@@ -212,106 +321,156 @@ __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
 // and the column sums (over rows) X1 = gate D u_p, X2 = gate D, X3 = g u, X4 = g, from which block_norm_cols_kernel makes the
 // gradients of the weights, biases and the channel gate.  Each workgroup leaves one partial per column, summed in a
 // fixed order afterwards: no atomics, the same bits on every run.
-template <int DT, bool VEC, bool BRANCH, bool PRE, int SUMS /* 0 none, 1 X1 X3, 2 all */>
-__global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
+template <typename COLS, bool FULL> struct BwdRow {
+    typename COLS::Raw branch, gate[FULL ? 1 : 0], d_hidden, residual, d_normed;
+    uint32_t gr;
+    u32x4 st;                            // the row's statistics
+};
+
+// SUMS: the column sums that are kept: 0 none, 1 X1 and X3, 2 all four (and the post norm's bias in z)
+template <int DT, bool VEC, bool BRANCH, bool PRE, bool FULL, int SUMS, bool PREFETCH, int MAXT, bool STREAM>
+__global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(NormArgs a) {
     typedef typename DType<DT>::T T_;
     __shared__ float sm[2 * 16 * 4];
     extern __shared__ float fold[];                      // (groups - 1) * T * 8 floats when SUMS > 0
     const int waves = a.T >> 6;
     const int group = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) / waves);
-    const Cols<DT, VEC> c = {(int)threadIdx.x - group * a.T, a.T, a.A};
+    const Cols<DT, VEC, STREAM> c = {(int)threadIdx.x - group * a.T, a.T, a.A};
     int slot = 0;
-    float pf[8], pb[8], qw[8];
+    const bool gated = a.gate_kind == MTC_GATE_ROW || a.gate_kind == MTC_GATE_SCALAR;
+    const long long base0 = (long long)blockIdx.x * a.groups, step = (long long)gridDim.x * a.groups;
+    typedef BwdRow<Cols<DT, VEC, STREAM>, FULL> Row;
+    auto fetch = [&](long long base, Row& q) {
+        const bool live = base + group < a.rows;
+        const long long row = live ? base + group : 0;
+        q.st = __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(a.stats, row * 16, live && a.stats ? 16 : 0), 0, 0, 0);
+        if (BRANCH) {
+            c.fetch(a.branch, row, live, q.branch);
+            c.fetch(a.d_hidden, row, live && a.d_hidden.p, q.d_hidden);
+            if (FULL) c.fetch(a.gate, row, live, q.gate[0]);
+            else q.gr = fetch_one<DT>(a.gate, row, live && gated);
+        }
+        if (PRE) {
+            c.fetch(a.residual, row, live, q.residual);
+            c.fetch(a.d_normed, row, live, q.d_normed);
+        }
+    };
+    Row first;
+    fetch(base0, first);
+    NormWeights w;
+    w.load(c, a, BRANCH, PRE);
     float x1[8], x2[8], x3[8], x4[8], gate_sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x1[i] = x2[i] = x3[i] = x4[i] = 0.f;
-    if (BRANCH) branch_factors(c, a, pf, pb);
-    if (PRE) c.weight(a.pre_w, a.pre_off, qw);
-    for (long long base = (long long)blockIdx.x * a.groups; base < a.rows; base += (long long)gridDim.x * a.groups) {
+    walk_rows<PREFETCH>(base0, step, a.rows, fetch, first, [&](long long base, const Row& q) {
+        // Groups behind the last row read zeros everywhere, 1/std among them: they add zeros and store nothing.
+        // The statistics are folded into the factors of fused multiply-adds, and work that only a layer norm, a row gate, a
+        // gate's gradient or a residual scale needs sits behind branches that the whole launch takes alike: the loop is
+        // bound by the number of vector instructions once the loads are in flight in time.
         const bool live = base + group < a.rows;
-        const long long row = live ? base + group : a.rows - 1;
-        float D[8], up[8], z[8], g[8], gr = 1.f, rstd_p = 1.f;
+        const long long row = live ? base + group : 0;
+        const float rstd_p = a.post_kind == MTC_NORM_NONE ? 1.f : __uint_as_float(q.st[1]);
+        const float gr = FULL || !gated ? 1.f : __uint_as_float(q.gr);
+        float D[8], up[8], z[8], g[8];
         if (BRANCH) {
-            c.load(a.branch.p, row * a.branch.ld, up);
-            if (a.gate_kind == MTC_GATE_FULL) c.load(a.gate.p, row * a.gate.ld, g);
-            if (a.gate_kind == MTC_GATE_ROW || a.gate_kind == MTC_GATE_SCALAR)
-                gr = DType<DT>::ld(reinterpret_cast<const T_*>(a.gate.p) + row * a.gate.ld);       // scalar: ld = 0
-            if (a.post_kind != MTC_NORM_NONE) {
-                const float mu_p = a.stats[row];
-                rstd_p = a.stats[a.rows + row];
+            q.branch.unpack(up);
+            if (a.post_kind == MTC_NORM_LAYER) {
+                const float k = -__uint_as_float(q.st[0]) * rstd_p;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) up[i] = (up[i] - mu_p) * rstd_p;
+                for (int i = 0; i < 8; ++i) up[i] = fmaf(up[i], rstd_p, k);
+            } else if (a.post_kind == MTC_NORM_RMS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) up[i] *= rstd_p;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = fmaf(up[i], pf[i], pb[i]);
-            if (a.gate_kind != MTC_GATE_FULL)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] = gr;
-            if (a.d_hidden.p) c.load(a.d_hidden.p, row * a.d_hidden.ld, D);
+            for (int i = 0; i < 8; ++i) z[i] = SUMS == 2 ? fmaf(up[i], w.pf[i], w.pb[i]) : up[i] * w.pf[i];
+            if (FULL) q.gate[0].unpack(g);
+            q.d_hidden.unpack(D);
         }
-        if (!BRANCH || !a.d_hidden.p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) D[i] = 0.f;
         if (PRE) {
-            float u[8], dn[8];
-            c.load(a.residual.p, row * a.residual.ld, u);
-            c.load(a.d_normed.p, row * a.d_normed.ld, dn);
-            const float mu = a.stats[2 * a.rows + row], rstd = a.stats[3 * a.rows + row];
-            float s[2] = {0.f, 0.f};
+            const float rstd = __uint_as_float(q.st[3]), k = -__uint_as_float(q.st[2]) * rstd;
+            const float kr = BRANCH ? a.res_scale * rstd : rstd, kz = gr * rstd;
+            float u[8], dn[8], s[2] = {0.f, 0.f};
+            q.residual.unpack(u);
+            q.d_normed.unpack(dn);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (BRANCH) u[i] = fmaf(g[i], z[i], a.res_scale * u[i]);
-                u[i] = (u[i] - mu) * rstd;
-                if (SUMS >= 1 && live) x3[i] = fmaf(dn[i], u[i], x3[i]);
-                if (SUMS >= 2 && live) x4[i] += dn[i];
-                dn[i] *= qw[i];
-                s[0] += dn[i];
-                s[1] = fmaf(dn[i], u[i], s[1]);
+                const float zi = BRANCH ? fmaf(FULL ? g[i] * rstd : kz, z[i], k) : k;
+                u[i] = fmaf(kr, u[i], zi);
+                if (SUMS >= 1) x3[i] = fmaf(dn[i], u[i], x3[i]);
+                if (SUMS >= 2) x4[i] += dn[i];
+                dn[i] *= w.qw[i];
+                s[0] = fmaf(dn[i], u[i], s[0]);
             }
-            group_sum(s, sm, slot, group, waves);
-            const float m1 = a.pre_kind == MTC_NORM_LAYER ? s[0] * a.inv_A : 0.f, m2 = s[1] * a.inv_A;
+            if (a.pre_kind == MTC_NORM_LAYER) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) D[i] = fmaf(rstd, dn[i] - m1 - u[i] * m2, D[i]);
+                for (int i = 0; i < 8; ++i) s[1] += dn[i];
+                group_sum(s, sm, slot, group, waves);
+                const float m1 = -s[1] * a.inv_A;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dn[i] += m1;
+            } else {
+                float s1[1] = {s[0]};
+                group_sum(s1, sm, slot, group, waves);
+                s[0] = s1[0];
+            }
+            const float m2 = -s[0] * a.inv_A * rstd;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) D[i] = fmaf(m2, u[i], BRANCH ? fmaf(rstd, dn[i], D[i]) : rstd * dn[i]);
         }
-        if (a.d_residual && live) {
+        if (BRANCH && a.res_scale != 1.f) {
             float o[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = BRANCH ? a.res_scale * D[i] : D[i];
-            c.store(a.d_residual, row * a.A, o);
+            for (int i = 0; i < 8; ++i) o[i] = a.res_scale * D[i];
+            c.store(a.d_residual, row, live && a.d_residual.p, o);
+        } else {
+            c.store(a.d_residual, row, live && a.d_residual.p, D);
         }
         if (BRANCH) {
             float s[3] = {0.f, 0.f, 0.f};
+            const bool row_sum = (a.gate_kind == MTC_GATE_ROW && a.d_gate.p) || a.want_scalar;
+            if (FULL || row_sum) {                       // d gate, before its reduction
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                z[i] *= D[i];                            // d gate, before its reduction
-                s[2] += z[i];
-            }
-            if (a.gate_kind == MTC_GATE_FULL && a.d_gate && live) c.store(a.d_gate, row * a.A, z);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                D[i] *= g[i];
-                if (SUMS >= 1 && live) x1[i] = fmaf(D[i], up[i], x1[i]);
-                if (SUMS >= 2 && live) x2[i] += D[i];
-                D[i] *= pf[i];
-                s[0] += D[i];
-                s[1] = fmaf(D[i], up[i], s[1]);
-            }
-            const bool row_gate = a.gate_kind == MTC_GATE_ROW && a.d_gate;
-            if (a.post_kind != MTC_NORM_NONE || row_gate || a.want_scalar) {
-                group_sum(s, sm, slot, group, waves);
-                if (row_gate && live && c.t == 0) DType<DT>::st(reinterpret_cast<T_*>(a.d_gate) + row, s[2]);
-                if (live) gate_sum += s[2];
-            }
-            if (a.d_branch && live) {
-                if (a.post_kind != MTC_NORM_NONE) {
-                    const float m1 = a.post_kind == MTC_NORM_LAYER ? s[0] * a.inv_A : 0.f, m2 = s[1] * a.inv_A;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) D[i] = rstd_p * (D[i] - m1 - up[i] * m2);
+                for (int i = 0; i < 8; ++i) {
+                    z[i] *= D[i];
+                    s[2] += z[i];
                 }
-                c.store(a.d_branch, row * a.A, D);
             }
+            if (FULL) c.store(a.d_gate, row, live && a.d_gate.p, z);
+            if (FULL || gated) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) D[i] *= FULL ? g[i] : gr;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (SUMS >= 1) x1[i] = fmaf(D[i], up[i], x1[i]);
+                if (SUMS >= 2) x2[i] += D[i];
+                D[i] *= w.pf[i];
+            }
+            if (a.post_kind != MTC_NORM_NONE) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[1] = fmaf(D[i], up[i], s[1]);
+            }
+            if (row_sum || a.post_kind == MTC_NORM_LAYER) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[0] += D[i];
+                group_sum(s, sm, slot, group, waves);
+                if (a.gate_kind == MTC_GATE_ROW && a.d_gate.p && live && c.t == 0)
+                    DType<DT>::st(reinterpret_cast<T_*>(a.d_gate.p) + row, s[2]);
+                gate_sum += s[2];
+            } else if (a.post_kind == MTC_NORM_RMS) {
+                float s1[1] = {s[1]};
+                group_sum(s1, sm, slot, group, waves);
+                s[1] = s1[0];
+            }
+            if (a.post_kind != MTC_NORM_NONE) {
+                const float m1 = a.post_kind == MTC_NORM_LAYER ? -s[0] * a.inv_A * rstd_p : 0.f, m2 = -s[1] * a.inv_A * rstd_p;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) D[i] = fmaf(m2, up[i], fmaf(rstd_p, D[i], m1));
+            }
+            c.store(a.d_branch, row, live && a.d_branch.p, D);
         }
-    }
+    });
     if constexpr (SUMS > 0) {
         // the groups' column sums folded through LDS, one partial per workgroup (vectors nobody asked for are skipped)
         float* out = a.partial + (size_t)blockIdx.x * (4 * a.pitch + 8);
@@ -335,7 +494,9 @@ __global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
                 for (int q = 1; q < a.groups; ++q)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] += fold[((q - 1) * 8 + i) * a.T + c.t];
-                Cols<MTC_F32, VEC>{c.t, c.T, c.A}.store(out + (size_t)which * a.pitch, 0, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c.in(i)) out[(size_t)which * a.pitch + c.col(i)] = x[i];
             }
         };
         put(x1, a.want_x1, 0);
@@ -423,6 +584,17 @@ static int norm_check(const mtc_block_norm_desc* d, const char* who) {
 
 static int norm_threads(int A) { return ((A + 7) / 8 + 63) / 64 * 64; }
 
+constexpr int NORM_BWD_T = 768;                    // threads of a backward workgroup, if a row needs no more: 168 registers each
+constexpr long long NORM_STREAM_BYTES = 256ll << 20;       // the Infinity Cache
+
+// workgroups for `want` row sets: at most per_cu on each CU, and every one the same number of rounds
+static unsigned norm_grid(long long want, int per_cu) {
+    const long long most = (long long)NORM_CUS * (per_cu < 1 ? 1 : per_cu);
+    if (want <= most) return (unsigned)want;
+    const long long rounds = (want + most - 1) / most;
+    return (unsigned)((want + rounds - 1) / rounds);
+}
+
 static int norm_elem(int dtype) { return dtype == MTC_BF16 ? 2 : 4; }
 
 static bool row_vec(const void* p, long long ld, long long rows, int dtype) {
@@ -450,7 +622,7 @@ static int norm_operands(const mtc_block_norm_desc* d, const char* who, const vo
 }
 
 static bool norm_inputs_vec(const mtc_block_norm_desc* d, const NormArgs& a) {
-    return (d->A & 7) == 0 && row_vec(a.residual.p, a.residual.ld, d->rows, d->dtype) &&
+    return (d->A & (16 / norm_elem(d->dtype) - 1)) == 0 && row_vec(a.residual.p, a.residual.ld, d->rows, d->dtype) &&
            row_vec(a.branch.p, a.branch.ld, d->rows, d->dtype) &&
            ((a.gate_kind != MTC_GATE_CHANNEL && a.gate_kind != MTC_GATE_FULL) ||
             row_vec(a.gate.p, a.gate_kind == MTC_GATE_FULL ? a.gate.ld : 0, d->rows, d->dtype)) &&
@@ -458,11 +630,20 @@ static bool norm_inputs_vec(const mtc_block_norm_desc* d, const NormArgs& a) {
            row_vec(a.pre_b, 0, 1, d->dtype);
 }
 
-template <int DT, bool VEC> static void launch_norm_fwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
-    const dim3 b(a.T * a.groups);
-    if (branch && a.pre_kind != MTC_NORM_NONE) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, true>), dim3(grid), b, 0, s, a);
-    else if (branch) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, false>), dim3(grid), b, 0, s, a);
-    else hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, false, true>), dim3(grid), b, 0, s, a);
+template <int DT, bool VEC, bool STREAM> static void launch_norm_fwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
+    const dim3 b(a.T * a.groups), g(grid);
+    const bool pre = a.pre_kind != MTC_NORM_NONE, full = a.gate_kind == MTC_GATE_FULL;
+    if (!branch) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, false, true, false, STREAM>), g, b, 0, s, a);
+    else if (pre && full) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, true, true, STREAM>), g, b, 0, s, a);
+    else if (pre) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, true, false, STREAM>), g, b, 0, s, a);
+    else if (full) hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, false, true, STREAM>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, false, false, STREAM>), g, b, 0, s, a);
+}
+
+template <int DT> static void launch_norm_fwd_dt(const NormArgs& a, bool branch, bool vec, bool stream, unsigned grid, hipStream_t s) {
+    if (!vec) launch_norm_fwd<DT, false, false>(a, branch, grid, s);
+    else if (stream) launch_norm_fwd<DT, true, true>(a, branch, grid, s);
+    else launch_norm_fwd<DT, true, false>(a, branch, grid, s);
 }
 
 extern "C" int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* residual, const void* branch, const void* gate,
@@ -478,6 +659,7 @@ extern "C" int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* resi
     MTC_REQUIRE((d->pre_kind == MTC_NORM_NONE) == !normed, "%s: normed pointer and pre_kind disagree", who);
     MTC_REQUIRE(d->rows <= 1 || ((!hidden || d->ld_hidden >= d->A) && (!normed || d->ld_normed >= d->A)),
                 "%s: output rows overlap (row stride below the width)", who);
+    MTC_REQUIRE(!stats || ((uintptr_t)stats & 15) == 0, "%s: stats must be 16-byte aligned", who);
     a.hidden = {hidden, d->ld_hidden};
     a.normed = {normed, d->ld_normed};
     a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.pre_b = pre_b;
@@ -485,22 +667,27 @@ extern "C" int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* resi
     const bool vec = norm_inputs_vec(d, a) && row_vec(hidden, d->ld_hidden, d->rows, d->dtype) &&
                      row_vec(normed, d->ld_normed, d->rows, d->dtype);
     a.groups = a.T >= 256 ? 1 : 256 / a.T;
-    const long long want = (d->rows + a.groups - 1) / a.groups;
-    const unsigned grid = (unsigned)(want < NORM_CUS * 8 ? want : NORM_CUS * 8);
+    // operands read and written once; beyond the Infinity Cache non-temporal accesses and, for two RMS norms (whose rows wait
+    // least), few waves that keep to few DRAM pages are faster: 16384 x 4608 bf16 pair 99 against 118 us, 65536 x 2304
+    // norm alone 109 against 115.  Within the cache the opposite holds: 4096 x 2304 pair 14.8 against 17.0 us, and what
+    // follows finds plain stores in the cache (four such calls in a row 60 against 65 us).
+    const int passes = (branch ? 2 : 1) + (d->gate_kind == MTC_GATE_FULL) + (hidden != nullptr) + (normed != nullptr);
+    const bool streaming = d->rows * d->A * norm_elem(d->dtype) * passes > NORM_STREAM_BYTES;
+    const bool layer = d->post_kind == MTC_NORM_LAYER || d->pre_kind == MTC_NORM_LAYER;
+    const int waves = !streaming ? 20 : branch && !layer ? 12 : 28;
+    const unsigned grid = norm_grid((d->rows + a.groups - 1) / a.groups, waves / (a.T * a.groups / 64));
     hipStream_t s = as_stream(stream);
-    if (d->dtype == MTC_BF16) vec ? launch_norm_fwd<MTC_BF16, true>(a, branch, grid, s) : launch_norm_fwd<MTC_BF16, false>(a, branch, grid, s);
-    else vec ? launch_norm_fwd<MTC_F32, true>(a, branch, grid, s) : launch_norm_fwd<MTC_F32, false>(a, branch, grid, s);
+    if (d->dtype == MTC_BF16) launch_norm_fwd_dt<MTC_BF16>(a, branch, vec, streaming, grid, s);
+    else launch_norm_fwd_dt<MTC_F32>(a, branch, vec, streaming, grid, s);
     return check_launch(who);
 }
 
 // backward launch shape: one workgroup per CU of up to 1024 threads, fewer row groups when there are few rows
 static void norm_bwd_shape(const mtc_block_norm_desc* d, int& groups, unsigned& grid) {
-    const int T = norm_threads(d->A);
+    const int T = norm_threads(d->A), most = T > NORM_BWD_T ? 1 : NORM_BWD_T / T;
     const long long per_cu = (d->rows + NORM_CUS - 1) / NORM_CUS;
-    groups = (int)(per_cu < 1024 / T ? per_cu : 1024 / T);
-    if (groups < 1) groups = 1;
-    const long long want = (d->rows + groups - 1) / groups;
-    grid = (unsigned)(want < NORM_CUS ? want : NORM_CUS);
+    groups = (int)(per_cu < most ? per_cu : most);
+    grid = norm_grid((d->rows + groups - 1) / groups, 1);
 }
 
 extern "C" size_t mtc_block_norm_bwd_workspace_bytes(const mtc_block_norm_desc* d) {
@@ -512,19 +699,31 @@ extern "C" size_t mtc_block_norm_bwd_workspace_bytes(const mtc_block_norm_desc* 
     return (size_t)grid * (4 * ((d->A + 7) / 8 * 8) + 8) * sizeof(float);
 }
 
-template <int DT, bool VEC, bool BRANCH, bool PRE>
-static void launch_norm_bwd(const NormArgs& a, int sums, unsigned grid, hipStream_t s) {
-    const dim3 b(a.T * a.groups);
+template <int DT, bool VEC, bool BRANCH, bool PRE, bool FULL, bool PREFETCH, int MAXT, bool STREAM>
+static void launch_norm_bwd_sums(const NormArgs& a, int sums, unsigned grid, hipStream_t s) {
+    const dim3 b(a.T * a.groups), g(grid);
     const size_t lds = sums ? (size_t)(a.groups - 1) * a.T * 8 * sizeof(float) : 0;
-    if (sums == 0) hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, 0>), dim3(grid), b, lds, s, a);
-    else if (sums == 1) hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, 1>), dim3(grid), b, lds, s, a);
-    else hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, 2>), dim3(grid), b, lds, s, a);
+    if (sums == 0) hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, FULL, 0, PREFETCH, MAXT, STREAM>), g, b, lds, s, a);
+    else if (VEC && sums == 1)
+        hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, FULL, VEC ? 1 : 2, PREFETCH, MAXT, STREAM>), g, b, lds, s, a);
+    else hipLaunchKernelGGL((block_norm_bwd_kernel<DT, VEC, BRANCH, PRE, FULL, 2, PREFETCH, MAXT, STREAM>), g, b, lds, s, a);
 }
 
-template <int DT, bool VEC> static void launch_norm_bwd_mode(const NormArgs& a, bool branch, int sums, unsigned grid, hipStream_t s) {
-    if (branch && a.pre_kind != MTC_NORM_NONE) launch_norm_bwd<DT, VEC, true, true>(a, sums, grid, s);
-    else if (branch) launch_norm_bwd<DT, VEC, true, false>(a, sums, grid, s);
-    else launch_norm_bwd<DT, VEC, false, true>(a, sums, grid, s);
+template <int DT, bool VEC, bool BRANCH, bool PRE, bool FULL>
+static void launch_norm_bwd(const NormArgs& a, int sums, bool streaming, unsigned grid, hipStream_t s) {
+    if (a.T * a.groups > NORM_BWD_T) launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, false, 1024, false>(a, sums, grid, s);
+    else if (VEC && !FULL && streaming) launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, VEC, NORM_BWD_T, VEC && !FULL>(a, sums, grid, s);
+    else launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, VEC, NORM_BWD_T, false>(a, sums, grid, s);
+}
+
+template <int DT, bool VEC>
+static void launch_norm_bwd_mode(const NormArgs& a, bool branch, int sums, bool streaming, unsigned grid, hipStream_t s) {
+    const bool pre = a.pre_kind != MTC_NORM_NONE, full = a.gate_kind == MTC_GATE_FULL;
+    if (!branch) launch_norm_bwd<DT, VEC, false, true, false>(a, sums, streaming, grid, s);
+    else if (pre && full) launch_norm_bwd<DT, VEC, true, true, true>(a, sums, streaming, grid, s);
+    else if (pre) launch_norm_bwd<DT, VEC, true, true, false>(a, sums, streaming, grid, s);
+    else if (full) launch_norm_bwd<DT, VEC, true, false, true>(a, sums, streaming, grid, s);
+    else launch_norm_bwd<DT, VEC, true, false, false>(a, sums, streaming, grid, s);
 }
 
 extern "C" int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* residual, const void* branch, const void* gate,
@@ -545,12 +744,15 @@ extern "C" int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* resi
     MTC_REQUIRE(d->post_kind != MTC_NORM_NONE || !(d_post_w || d_post_b), "%s: gradient of an absent post norm", who);
     MTC_REQUIRE(d->gate_kind != MTC_GATE_NONE || !d_gate, "%s: gradient of an absent gate", who);
     MTC_REQUIRE(stats || (d->pre_kind == MTC_NORM_NONE && d->post_kind == MTC_NORM_NONE), "%s: null stats", who);
+    MTC_REQUIRE(!stats || ((uintptr_t)stats & 15) == 0, "%s: stats must be 16-byte aligned", who);
     MTC_REQUIRE(ld_d_hidden >= 0 && ld_d_normed >= 0, "%s: negative row stride", who);
     a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.pre_b = pre_b;
     a.stats = const_cast<float*>(stats);
     a.d_hidden = {const_cast<void*>(d_hidden), ld_d_hidden};
     a.d_normed = {const_cast<void*>(d_normed), ld_d_normed};
-    a.d_residual = d_residual; a.d_branch = d_branch; a.d_gate = d_gate;
+    a.d_residual = {d_residual, d->A};
+    a.d_branch = {d_branch, d->A};
+    a.d_gate = {d_gate, d->A};
     const bool chan = d->gate_kind == MTC_GATE_CHANNEL && d_gate;
     const bool chan_bias = chan && d->post_kind != MTC_NORM_NONE && post_b;
     a.want_x1 = d_post_w || chan;
@@ -558,11 +760,13 @@ extern "C" int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* resi
     a.want_x3 = d_pre_w != nullptr;
     a.want_x4 = d_pre_b != nullptr;
     a.want_scalar = d->gate_kind == MTC_GATE_SCALAR && d_gate;
-    const int sums = a.want_x2 || a.want_x4 ? 2 : a.want_x1 || a.want_x3 || a.want_scalar ? 1 : 0;
+    const bool any_sum = a.want_x1 || a.want_x2 || a.want_x3 || a.want_x4 || a.want_scalar;
+    // 2: also whenever the branch's norm has a bias, which the smaller forms leave out of the recomputed branch
+    const int sums = a.want_x2 || a.want_x4 || (d->post_kind != MTC_NORM_NONE && post_b) ? 2 : any_sum ? 1 : 0;
     a.pitch = (d->A + 7) / 8 * 8;
     unsigned grid;
     norm_bwd_shape(d, a.groups, grid);
-    if (sums) {
+    if (any_sum) {
         MTC_REQUIRE(workspace && workspace_bytes >= mtc_block_norm_bwd_workspace_bytes(d), "%s: workspace too small", who);
         MTC_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned", who);
         a.partial = reinterpret_cast<float*>(workspace);
@@ -573,12 +777,17 @@ extern "C" int mtc_block_norm_bwd(const mtc_block_norm_desc* d, const void* resi
                      row_vec(d_branch, A, d->rows, d->dtype) &&
                      (d->gate_kind != MTC_GATE_FULL || row_vec(d_gate, A, d->rows, d->dtype));
     hipStream_t s = as_stream(stream);
+    // non-temporal beyond the Infinity Cache: 16384 x 4608 bf16 pair 158 against 174 us; 1024 x 768 fp32, within it: 12.4
+    // against 10.8 us
+    const int passes = (branch ? 1 : 0) + (d_hidden != nullptr) + (d->pre_kind != MTC_NORM_NONE ? 2 : 0) + (d_residual != nullptr) +
+                       (d_branch != nullptr);
+    const bool streaming = d->rows * A * norm_elem(d->dtype) * passes > NORM_STREAM_BYTES;
     if (d->dtype == MTC_BF16)
-        vec ? launch_norm_bwd_mode<MTC_BF16, true>(a, branch, sums, grid, s) : launch_norm_bwd_mode<MTC_BF16, false>(a, branch, sums, grid, s);
+        vec ? launch_norm_bwd_mode<MTC_BF16, true>(a, branch, sums, streaming, grid, s) : launch_norm_bwd_mode<MTC_BF16, false>(a, branch, sums, streaming, grid, s);
     else
-        vec ? launch_norm_bwd_mode<MTC_F32, true>(a, branch, sums, grid, s) : launch_norm_bwd_mode<MTC_F32, false>(a, branch, sums, grid, s);
+        vec ? launch_norm_bwd_mode<MTC_F32, true>(a, branch, sums, streaming, grid, s) : launch_norm_bwd_mode<MTC_F32, false>(a, branch, sums, streaming, grid, s);
     if (check_launch(who)) return -2;
-    if (sums) {
+    if (any_sum) {
         NormCols n = {};
         n.A = d->A; n.parts = (int)grid; n.pitch = a.pitch; n.gate_kind = d->gate_kind;
         n.branch_scale = d->branch_scale; n.post_off = d->post_offset;

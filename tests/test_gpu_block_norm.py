@@ -219,6 +219,45 @@ def test_partial_gradients(dt):
     N.compare("residual", gr, N.reference(res, br, None, _spec(post), _spec(pre), 1.0, 1.0, d, d)["residual"], dt)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_frozen_norms_with_bias(dt):
+    """Frozen layer norms: their biases still belong to the recomputed sum that the pre norm's gradient is taken at."""
+    g = torch.Generator("cpu").manual_seed(17)
+    rows, A = 70, 264
+    post, pre = _norm_module(g, A, "layer", dt).requires_grad_(False), _norm_module(g, A, "layer", dt).requires_grad_(False)
+    for gate_kind in ("none", "channel", "full", "scalar"):
+        res, br = _rand(g, rows, A).to(dt).to(DEV).requires_grad_(True), _rand(g, rows, A).to(dt).to(DEV).requires_grad_(True)
+        gate, d = _gate(g, gate_kind, rows, A, dt), _rand(g, rows, A).to(dt).to(DEV)
+        out = residual_block_norm(res, br, post, gate=gate, pre=pre)
+        want = N.reference(res, br, gate, _spec(post), _spec(pre), 1.0, 1.0, d, d)
+        for k, v in zip(("residual", "branch"), torch.autograd.grad(out, [res, br], [d, d])):
+            N.compare(k, v, want[k], dt)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_streaming_sizes(dt):
+    """Passes over more than the Infinity Cache holds run with non-temporal accesses: the same bits as row blocks within it."""
+    g = torch.Generator("cpu").manual_seed(18)
+    rows, A = (34000, 2304) if dt == torch.bfloat16 else (17000, 2304)
+    gen = torch.Generator(DEV).manual_seed(18)
+    res, br, dh, dn = (torch.randn(rows, A, generator=gen, device=DEV).to(dt) for _ in range(4))
+    post, pre = _norm_module(g, A, "rms", dt), _norm_module(g, A, "rms", dt)
+
+    def both(lo, hi):
+        r, b = res[lo:hi].detach().requires_grad_(True), br[lo:hi].detach().requires_grad_(True)
+        out = residual_block_norm(r, b, post, pre=pre)
+        return list(out) + list(torch.autograd.grad(out, [r, b, post.weight], [dh[lo:hi], dn[lo:hi]]))
+
+    whole = both(0, rows)
+    for lo in range(0, rows, 4000):
+        part = both(lo, min(rows, lo + 4000))
+        for a, b in zip(whole[:4], part[:4]):
+            assert torch.equal(a[lo:lo + 4000], b)
+    N.compare("post_w", whole[4], N.reference(res, br, None, _spec(post), _spec(pre), 1.0, 1.0, dh, dn)["post_w"], dt)
+    alone = block_norm(res, pre.weight, eps=1e-6, weight_offset=1.0)
+    assert torch.equal(alone[1000:2000], block_norm(res[1000:2000], pre.weight, eps=1e-6, weight_offset=1.0))
+
+
 def test_gradient_against_differences():
     """<gradient, v> against central differences of the float64 forward along v."""
     g = torch.Generator("cpu").manual_seed(14)
