@@ -8,7 +8,18 @@ LIB   := matryoshka_transcoder_amd/libmtc.so
 # no packed fp32 instructions: the compiler forms them from plain float code, and some of their forms are not reliable here
 FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
 
-all: $(LIB)
+# host side of the block norms and the gradient clipping on torch tensors (no kernels; calls libmtc.so by address)
+BINDING := matryoshka_transcoder_amd/_torch_binding.so
+PYTHON  ?= python3
+TORCH    = $(shell $(PYTHON) -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+PYINC    = $(shell $(PYTHON) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+
+all: $(LIB) $(BINDING)
+
+$(BINDING): $(CSRC)/torch_binding.cpp include/mtc.h
+	$(CXX) -std=c++17 -O2 -Wall -fPIC -shared -fvisibility=hidden -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -Iinclude \
+		-isystem $(TORCH)/include -isystem $(TORCH)/include/torch/csrc/api/include -isystem $(PYINC) -isystem /opt/rocm/include \
+		$< -o $@ -L$(TORCH)/lib -lc10 -lc10_hip -ltorch_cpu -ltorch_python
 
 $(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/common.hpp $(CSRC)/rowops.hpp include/mtc.h
 	$(HIPCC) $(FLAGS) -c $< -o $@
@@ -17,6 +28,6 @@ $(LIB): $(OBJS)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC -o $@ $(OBJS) -ldl
 
 clean:
-	rm -f $(OBJS) $(LIB)
+	rm -f $(OBJS) $(LIB) $(BINDING)
 
 .PHONY: all clean

@@ -163,6 +163,26 @@ def load() -> C.CDLL:
     return lib
 
 
+_BINDING = None
+
+
+def torch_binding():
+    """The C++ host side of the block norms and the gradient clipping (csrc/torch_binding.cpp, built in-tree by `make`),
+    bound to the library that `load` opened.  Raises MtcError if it is absent -- there is no other path."""
+    global _BINDING
+    if _BINDING is None:
+        lib = load()
+        try:
+            from . import _torch_binding
+        except ImportError as e:
+            raise MtcError(f"matryoshka_transcoder_amd/_torch_binding.so could not be loaded ({e}): build it with `make`") from None
+        _torch_binding.bind({name: C.cast(getattr(lib, name), P).value for name in
+                             ("mtc_last_error", "mtc_block_norm_fwd", "mtc_block_norm_bwd", "mtc_block_norm_bwd_workspace_bytes",
+                              "mtc_grad_norm_workspace_bytes", "mtc_grad_norm", "mtc_grad_clip")}, MtcError)
+        _BINDING = _torch_binding
+    return _BINDING
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = load().mtc_last_error()

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from matryoshka_transcoder_amd import _lib
-from matryoshka_transcoder_amd.grad_clip import _dense, clip_by_global_norm_, clip_grad_norm_, global_norm, norm_and_coef
+from matryoshka_transcoder_amd.grad_clip import clip_by_global_norm_, clip_grad_norm_, global_norm, norm_and_coef
 
 GOOD = 0x10000
 
@@ -96,11 +96,3 @@ def test_python_refusals():
             clip_by_global_norm_([], m)
     assert float(global_norm([])) == 0.0 and float(clip_by_global_norm_([], 1.0, math.inf)) == 0.0
     assert float(clip_grad_norm_([torch.nn.Parameter(t)], 1.0)) == 0.0           # no .grad anywhere
-
-
-def test_dense_views():
-    x = torch.zeros(4, 6, 8)
-    for t, want in ((x, True), (x.t() if x.dim() == 2 else x.permute(2, 0, 1), True), (x[:, :3], False), (x[..., ::2], False),
-                    (x[0], True), (x[:, :1].squeeze(1), False), (torch.zeros(1, 5).expand(3, 5), False), (torch.zeros(()), True),
-                    (torch.zeros(3, 0), True), (torch.zeros(5, 1).t(), True), (torch.as_strided(torch.zeros(9), (3, 3), (2, 2)), False)):
-        assert _dense(t) is want, (t.shape, t.stride())
