@@ -4,11 +4,17 @@
 // Bound by memory: the norm reads every gradient once, the scaling reads and writes it once more.
 //
 // The list of tensors travels in the kernel arguments (128 per launch): nothing is copied to the device, so a captured
-// launch carries its own list.  A tile is 32 KiB of one tensor; workgroups walk over the tiles of all tensors, each keeps one
-// running sum and leaves one partial.  Sums are held in 64 bits: a dictionary's gradient has 10^8 elements, and squares of
-// fp32 values leave the range of fp32.  The partials are added in a fixed order (no atomics: the same bits on every run) by
-// whoever needs the norm: a one-workgroup launch, or every workgroup of the scaling launch for itself, which saves that
-// launch and its wait.
+// launch carries its own list.  A tile is 16 KiB of one tensor.  For the norm, workgroups walk over the tiles of all tensors, each
+// keeps one running sum and leaves one partial.  Sums are held in 64 bits: a dictionary's gradient has 10^8 elements, and
+// squares of fp32 values leave the range of fp32; squaring in fp32 instead measured no faster (60 us for 340 MB either
+// way).  The partials are added in a fixed order (no atomics: the same bits on every run).
+//
+// Scaling.  Up to SMALL_TILES tiles every workgroup adds up the partials for itself, which saves a launch and its wait (61
+// tensors of 5 KiB 11 against 15 us, 75 MB 38 against 39); beyond, one workgroup does it once and each tile gets a
+// workgroup of its own (1.36 GB 672 against 731 us: neighbouring workgroups then share DRAM pages).  It walks from the
+// last tile to the first, because the norm's pass has left the last ones in the Infinity Cache.  Stores are
+// non-temporal (340 MB 156 against 190 us; an Adam update right behind is no slower for it), loads only when the list is
+// well beyond that cache (1.36 GB 648 against 672 us; 340 MB 161 against 156).
 #include <algorithm>
 #include <new>
 #include "common.hpp"
@@ -16,8 +22,11 @@
 namespace mtc {
 
 constexpr int CLIP_BATCH = 128;            // tensors per launch (kernel arguments are limited to 4 KiB)
-constexpr int TILE_UNITS = 2048;           // 16-byte units per tile: 8 per thread
-constexpr int CLIP_GRID = 2048;            // workgroups of one launch
+constexpr int TILE_UNITS = 1024;           // 16-byte units per tile: 4 per thread
+constexpr int PER_THREAD = TILE_UNITS / 256;
+constexpr int CLIP_GRID = 2048;            // workgroups of one launch that walk over tiles
+constexpr int SMALL_TILES = 8192;          // 128 MiB
+constexpr uint64_t STREAM_TILES = 32768;   // 512 MiB: twice the Infinity Cache
 constexpr float CLIP_EPS = 1e-6f;
 
 enum { POW_1 = 1, POW_2 = 2, POW_INF = 3 };
@@ -103,7 +112,12 @@ template <int DT> __device__ __forceinline__ u32x4 unit_pack(const float (&v)[DT
     return r;
 }
 
-template <int DT, int POW>
+template <bool STREAM> __device__ __forceinline__ u32x4 load_unit(const u32x4* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
+template <int DT, int POW, bool STREAM>
 __device__ __forceinline__ void sum_tile(const void* src, uint64_t n, bool aligned, uint64_t local, Acc<POW>& acc) {
     typedef typename DType<DT>::T T;
     constexpr int E = DType<DT>::kVec;
@@ -111,11 +125,11 @@ __device__ __forceinline__ void sum_tile(const void* src, uint64_t n, bool align
     const uint64_t e0 = local * (uint64_t)(TILE_UNITS * E);
     if (aligned && e0 + TILE_UNITS * E <= n) {
         const u32x4* q = reinterpret_cast<const u32x4*>(p + e0) + threadIdx.x;
-        u32x4 r[8];
+        u32x4 r[PER_THREAD];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) r[k] = q[k * 256];
+        for (int k = 0; k < PER_THREAD; ++k) r[k] = load_unit<STREAM>(q + k * 256);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < PER_THREAD; ++k) {
             float v[E];
             unit_values<DT>(r[k], v);
 #pragma unroll
@@ -138,7 +152,7 @@ __device__ __forceinline__ void sum_tile(const void* src, uint64_t n, bool align
     for (i += threadIdx.x; i < end; i += 256) acc.add(DType<DT>::ld(p + i));
 }
 
-template <int POW>
+template <int POW, bool STREAM>
 __global__ __launch_bounds__(256) void power_sum_kernel(ClipBatch b, double* __restrict__ partial) {
     __shared__ double sm[4];
     Acc<POW> acc;
@@ -146,29 +160,31 @@ __global__ __launch_bounds__(256) void power_sum_kernel(ClipBatch b, double* __r
         const int t = tensor_of(b, tile);
         const uint64_t n = b.elems[t] & ELEM_MASK;
         const bool aligned = (b.elems[t] >> 62) & 1;
-        if (b.elems[t] >> 63) sum_tile<MTC_BF16, POW>(b.src[t], n, aligned, tile - b.first[t], acc);
-        else sum_tile<MTC_F32, POW>(b.src[t], n, aligned, tile - b.first[t], acc);
+        if (b.elems[t] >> 63) sum_tile<MTC_BF16, POW, STREAM>(b.src[t], n, aligned, tile - b.first[t], acc);
+        else sum_tile<MTC_F32, POW, STREAM>(b.src[t], n, aligned, tile - b.first[t], acc);
     }
     const double v = block_join<POW>(acc.value(), sm);
     if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
-// the partials' total: as it is (to be added up over ranks), or as {norm, coef}
+// the partials' total: as it is (to be added up over ranks), as {norm, coef}, as the norm
 template <int POW>
 __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restrict__ partial, int parts, float max_norm,
-                                                          double* __restrict__ total, float* __restrict__ norm_coef) {
+                                                          double* __restrict__ total, float* __restrict__ norm_coef,
+                                                          float* __restrict__ norm_out) {
     __shared__ double sm[4];
     const double v = join_partials<POW>(partial, parts, sm);
     if (threadIdx.x) return;
+    const float norm = root<POW>(v);
     if (total) *total = v;
     if (norm_coef) {
-        const float norm = root<POW>(v);
         norm_coef[0] = norm;
         norm_coef[1] = clip_coef(norm, max_norm);
     }
+    if (norm_out) *norm_out = norm;
 }
 
-template <int DT>
+template <int DT, bool STREAM>
 __device__ __forceinline__ void scale_tile(const void* src, void* dst, uint64_t n, bool aligned, uint64_t local, float coef) {
     typedef typename DType<DT>::T T;
     constexpr int E = DType<DT>::kVec;
@@ -178,16 +194,16 @@ __device__ __forceinline__ void scale_tile(const void* src, void* dst, uint64_t 
     if (aligned && e0 + TILE_UNITS * E <= n) {
         const u32x4* q = reinterpret_cast<const u32x4*>(p + e0) + threadIdx.x;
         u32x4* w = reinterpret_cast<u32x4*>(o + e0) + threadIdx.x;
-        u32x4 r[8];
+        u32x4 r[PER_THREAD];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) r[k] = q[k * 256];
+        for (int k = 0; k < PER_THREAD; ++k) r[k] = load_unit<STREAM>(q + k * 256);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < PER_THREAD; ++k) {
             float v[E];
             unit_values<DT>(r[k], v);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] *= coef;
-            w[k * 256] = unit_pack<DT>(v);
+            __builtin_nontemporal_store(unit_pack<DT>(v), w + k * 256);
         }
         return;
     }
@@ -207,22 +223,35 @@ __device__ __forceinline__ void scale_tile(const void* src, void* dst, uint64_t 
     for (i += threadIdx.x; i < end; i += 256) DType<DT>::st(o + i, DType<DT>::ld(p + i) * coef);
 }
 
+template <bool STREAM>
+__device__ __forceinline__ void scale_tiles(const ClipBatch& b, uint32_t k, uint32_t step, float coef) {
+    for (; k < (uint32_t)b.tiles; k += step) {
+        const uint32_t tile = b.tiles - 1 - k;           // last tiles first
+        const int t = tensor_of(b, tile);
+        const uint64_t n = b.elems[t] & ELEM_MASK;
+        const bool aligned = (b.elems[t] >> 62) & 1;
+        if (b.elems[t] >> 63) scale_tile<MTC_BF16, STREAM>(b.src[t], b.dst[t], n, aligned, tile - b.first[t], coef);
+        else scale_tile<MTC_F32, STREAM>(b.src[t], b.dst[t], n, aligned, tile - b.first[t], coef);
+    }
+}
+
+// in place and coef 1: nothing would change, g * 1 is g bit for bit
 template <int POW>
-__global__ __launch_bounds__(256) void clip_kernel(ClipBatch b, const double* __restrict__ partial, int parts, float max_norm,
-                                                   int in_place, float* __restrict__ norm_out) {
+__global__ __launch_bounds__(256) void clip_small_kernel(ClipBatch b, const double* __restrict__ partial, int parts, float max_norm,
+                                                         int in_place, float* __restrict__ norm_out) {
     __shared__ double sm[4];
     const float norm = root<POW>(join_partials<POW>(partial, parts, sm));
     const float coef = clip_coef(norm, max_norm);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-    if (in_place && coef == 1.f) return;                 // nothing would change: g * 1 is g, bit for bit
-    for (uint32_t k = blockIdx.x; k < (uint32_t)b.tiles; k += gridDim.x) {
-        const uint32_t tile = b.tiles - 1 - k;           // last tiles first: the norm's pass left them in the caches
-        const int t = tensor_of(b, tile);
-        const uint64_t n = b.elems[t] & ELEM_MASK;
-        const bool aligned = (b.elems[t] >> 62) & 1;
-        if (b.elems[t] >> 63) scale_tile<MTC_BF16>(b.src[t], b.dst[t], n, aligned, tile - b.first[t], coef);
-        else scale_tile<MTC_F32>(b.src[t], b.dst[t], n, aligned, tile - b.first[t], coef);
-    }
+    if (in_place && coef == 1.f) return;
+    scale_tiles<false>(b, blockIdx.x, gridDim.x, coef);
+}
+
+template <bool STREAM>
+__global__ __launch_bounds__(256) void clip_large_kernel(ClipBatch b, const float* __restrict__ norm_coef, int in_place) {
+    const float coef = norm_coef[1];
+    if (in_place && coef == 1.f) return;
+    scale_tiles<STREAM>(b, blockIdx.x, gridDim.x, coef);
 }
 
 template <int POW> __global__ void norm_coef_kernel(const double* __restrict__ total, float max_norm, float* __restrict__ norm_coef) {
@@ -315,26 +344,32 @@ static int clip_parts(const ClipList& l) {
     return parts;
 }
 
+static uint64_t clip_tiles(const ClipList& l) {
+    uint64_t tiles = 0;
+    for (int i = 0; i < l.n; ++i) {
+        const uint64_t per = (uint64_t)TILE_UNITS * (l.dtype[i] == MTC_BF16 ? 8 : 4);
+        tiles += (l.elems[i] + per - 1) / per;
+    }
+    return tiles;
+}
+
 extern "C" size_t mtc_grad_norm_workspace_bytes(int32_t n, const uint64_t* elems, const int32_t* dtype) {
     if (n < 0 || (n && (!elems || !dtype))) return 0;
-    // parts of any batch <= its tiles <= sum of ceil(bytes / 32 KiB); capped per launch of up to 128 tensors
-    uint64_t tiles = 0;
-    for (int i = 0; i < n; ++i) {
-        const uint64_t per = (uint64_t)TILE_UNITS * (dtype[i] == MTC_BF16 ? 8 : 4);
-        tiles += (elems[i] + per - 1) / per;
-    }
+    // one partial per workgroup of the norm's launches (each at most its tiles, and CLIP_GRID), then {norm, coef}
+    const uint64_t tiles = clip_tiles({n, nullptr, nullptr, elems, dtype});
     const uint64_t cap = (uint64_t)CLIP_GRID * ((n + CLIP_BATCH - 1) / CLIP_BATCH + 1);
     return (size_t)(std::min(tiles, cap) + 1) * sizeof(double);
 }
 
-template <int POW> static int sum_launch(const ClipList& l, double* partial, hipStream_t s) {
+template <int POW> static int sum_launch(const ClipList& l, double* partial, bool streaming, hipStream_t s) {
     int parts = 0;
     ClipBatch b;
     for (int i = 0; i < l.n;) {
         i = clip_batch(l, i, b);
         if (!b.tiles) continue;
         const int grid = std::min(b.tiles, CLIP_GRID);
-        hipLaunchKernelGGL(power_sum_kernel<POW>, dim3(grid), dim3(256), 0, s, b, partial + parts);
+        if (streaming) hipLaunchKernelGGL((power_sum_kernel<POW, true>), dim3(grid), dim3(256), 0, s, b, partial + parts);
+        else hipLaunchKernelGGL((power_sum_kernel<POW, false>), dim3(grid), dim3(256), 0, s, b, partial + parts);
         parts += grid;
     }
     return parts;
@@ -342,26 +377,32 @@ template <int POW> static int sum_launch(const ClipList& l, double* partial, hip
 
 template <int POW>
 static void norm_launch(const ClipList& l, double* ws, double* total, float max_norm, float* norm_coef, hipStream_t s) {
-    const int parts = sum_launch<POW>(l, ws, s);
-    hipLaunchKernelGGL(norm_finish_kernel<POW>, dim3(1), dim3(256), 0, s, ws, parts, max_norm, total, norm_coef);
+    const int parts = sum_launch<POW>(l, ws, clip_tiles(l) > STREAM_TILES, s);
+    hipLaunchKernelGGL(norm_finish_kernel<POW>, dim3(1), dim3(256), 0, s, ws, parts, max_norm, total, norm_coef, (float*)nullptr);
 }
 
 template <int POW> static void clip_launch(const ClipList& l, double* ws, float max_norm, float* norm_out, hipStream_t s) {
-    const int parts = sum_launch<POW>(l, ws, s);
-    bool wrote = false;
+    const uint64_t tiles = clip_tiles(l);
+    const bool streaming = tiles > STREAM_TILES, small = tiles <= SMALL_TILES;
+    const int parts = sum_launch<POW>(l, ws, streaming, s);
+    float* norm_coef = reinterpret_cast<float*>(ws + parts);
+    if (!small || !tiles)
+        hipLaunchKernelGGL(norm_finish_kernel<POW>, dim3(1), dim3(256), 0, s, ws, parts, max_norm, (double*)nullptr, norm_coef, norm_out);
     ClipBatch b;
     for (int i = 0; i < l.n;) {
         i = clip_batch(l, i, b);
         if (!b.tiles) continue;
         int in_place = 1;
         for (int t = 0; t < b.n; ++t) in_place &= b.src[t] == b.dst[t];
-        hipLaunchKernelGGL(clip_kernel<POW>, dim3(std::min(b.tiles, CLIP_GRID)), dim3(256), 0, s, b, ws, parts, max_norm, in_place,
-                           wrote ? nullptr : norm_out);
-        wrote = true;
-    }
-    if (!wrote && norm_out) {                                     // nothing but empty tensors: norm 0
-        b.n = b.tiles = 0;
-        hipLaunchKernelGGL(clip_kernel<POW>, dim3(1), dim3(256), 0, s, b, ws, 0, max_norm, 1, norm_out);
+        if (small) {
+            hipLaunchKernelGGL(clip_small_kernel<POW>, dim3(std::min(b.tiles, CLIP_GRID)), dim3(256), 0, s, b, ws, parts, max_norm, in_place,
+                               norm_out);
+            norm_out = nullptr;                          // the first launch has written it
+        } else if (streaming) {
+            hipLaunchKernelGGL(clip_large_kernel<true>, dim3(b.tiles), dim3(256), 0, s, b, norm_coef, in_place);
+        } else {
+            hipLaunchKernelGGL(clip_large_kernel<false>, dim3(b.tiles), dim3(256), 0, s, b, norm_coef, in_place);
+        }
     }
 }
 
@@ -373,7 +414,7 @@ extern "C" int mtc_grad_norm(int32_t n, const void* const* grads, const uint64_t
     if (clip_check(l, p, who)) return -1;
     MTC_REQUIRE(total || norm_coef, "%s: no output", who);
     MTC_REQUIRE(max_norm >= 0.f, "%s: max_norm must not be negative or NaN", who);
-    MTC_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= (size_t)clip_parts(l) * sizeof(double),
+    MTC_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= (size_t)(clip_parts(l) + 1) * sizeof(double),
                 "%s: workspace missing, misaligned or too small", who);
     double* ws = reinterpret_cast<double*>(workspace);
     hipStream_t s = as_stream(stream);
@@ -403,7 +444,7 @@ extern "C" int mtc_grad_clip(int32_t n, const void* const* grads, void* const* o
     MTC_REQUIRE(n <= 0 || out, "%s: null output list", who);
     if (clip_check(l, p, who) || clip_check_overlap(l, who)) return -1;
     MTC_REQUIRE(max_norm >= 0.f, "%s: max_norm must not be negative or NaN", who);
-    MTC_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= (size_t)clip_parts(l) * sizeof(double),
+    MTC_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= (size_t)(clip_parts(l) + 1) * sizeof(double),
                 "%s: workspace missing, misaligned or too small", who);
     double* ws = reinterpret_cast<double*>(workspace);
     hipStream_t s = as_stream(stream);

@@ -154,6 +154,18 @@ def test_non_finite(p, dt):
             assert torch.equal(torch.isnan(r.grad), torch.isnan(t)) and torch.equal(torch.nan_to_num(r.grad), torch.nan_to_num(t.float()))
 
 
+@pytest.mark.parametrize("mb", [100, 130, 300, 600])
+def test_large_lists(mb):
+    """Either side of the sizes at which the launches change: whole values, in place and into outputs, and a limit that is
+    not reached."""
+    n = mb * 250_000                                                   # fp32 + bf16 tensors of together mb MB
+    g = torch.Generator(DEV).manual_seed(mb)
+    ts = [torch.randn(n // 2 + 5, generator=g, device=DEV), torch.randn(n - 3, generator=g, device=DEV).bfloat16(), torch.ones(3, device=DEV)]
+    _check(ts, 1e9, 2.0)
+    _check(ts, 10.0, 2.0, out=[torch.empty_like(t) for t in ts])
+    _check(ts, 10.0, 2.0)
+
+
 def test_offsets_beyond_32_bits():
     n = (1 << 31) + 16400
     t = torch.zeros(n, dtype=torch.bfloat16, device=DEV)

@@ -77,8 +77,8 @@ def test_workspace_covers_any_list():
         live = [e for e in elems if e]
         parts = 0
         for i in range(0, len(live), 128):
-            parts += min(2048, sum((e + 16383) // 16384 for e in live[i:i + 128]))
-        assert lib.mtc_grad_norm_workspace_bytes(len(elems), el, dt) >= 8 * parts
+            parts += min(2048, sum((e + 8191) // 8192 for e in live[i:i + 128]))
+        assert lib.mtc_grad_norm_workspace_bytes(len(elems), el, dt) >= 8 * (parts + 1)
 
 
 def test_python_refusals():
