@@ -63,7 +63,11 @@ class TensorPairSource:
 
 class TranscoderActivationsStore:
     def __init__(self, model, cfg: dict, source=None, token_iterator: Optional[Iterator] = None):
+        """cfg["source_norm"] (optional, a block_norm.BlockNorm on the GPU): the harvested source is the residual stream in
+        front of a block, and the block's own norm of it becomes the transcoder's source activation -- one stream to
+        harvest or store instead of two, for models that have no hook behind that norm."""
         self.model = model
+        self.source_norm = cfg.get("source_norm")
         self.config = cfg
         self.device = cfg["device"]
         self.source_hook_point = cfg.get("source_hook_point")
@@ -113,7 +117,13 @@ class TranscoderActivationsStore:
         dt = self.config.get("dtype")
         if dt is not None:
             src, tgt = src.to(dtype=dt), tgt.to(dtype=dt)
-        return src, tgt
+        return self._normed(src), tgt
+
+    def _normed(self, src):
+        if self.source_norm is None:
+            return src
+        with torch.no_grad():
+            return self.source_norm(src)
 
     def get_batch_with_tokens(self):
         toks = self.get_batch_tokens()
@@ -128,6 +138,7 @@ class TranscoderActivationsStore:
         for _ in range(self.num_batches_in_buffer):
             if self.source is not None:
                 s, t = self.source.next_chunk(self.device, self.config["dtype"])
+                s = self._normed(s)
             else:
                 s, t = self.get_paired_activations(self.get_batch_tokens())
             srcs.append(s.reshape(-1, a_s))

@@ -259,6 +259,28 @@ class HotPath:
                                       _p(d_vals), float(l1_term), _stream()), "mtc_decode_fwd")
         return x_hat, g, row_stats, recons, d_vals
 
+    def reconstruct(self, sel: Selection, W_dec, b_dec, rows: int, mean=None, std=None):
+        """a15: pure decode of a selection, de-normalised when mean / std [rows] are given."""
+        _need(W_dec, "W_dec", self.dtype, (self.D, self.A_t))
+        _need(b_dec, "b_dec", self.dtype, (self.A_t,))
+        d = _lib.make_desc(rows, self.A_s, self.A_t, self.D, self.prefix, self.code, mean is not None)
+        x_hat = torch.empty(rows, self.A_t, dtype=self.dtype, device=W_dec.device)
+        check(self.lib.mtc_decode_fwd(C.byref(d), _p(sel.row_ptr), _p(sel.col_idx), _p(sel.vals), _p(W_dec), _p(b_dec), None,
+                                      _p(mean), _p(std), _p(x_hat), None, None, None, None, 0.0, _stream()), "mtc_decode_fwd")
+        return x_hat
+
+    def encoder_input_grad(self, sel: Selection, d_vals, W_encT, rows: int):
+        """Gradient of the encoder's input: sum_j d a_bj W_encT[j] over the selected entries, i.e. the same gather as a pure
+        decode, with the encoder's rows and no bias.  d_vals hold values of the model dtype."""
+        _need(W_encT, "W_encT", self.dtype, (self.D, self.A_s))
+        d = _lib.make_desc(rows, self.A_t, self.A_s, self.D, [self.D], self.code, False)
+        dx = torch.empty(rows, self.A_s, dtype=self.dtype, device=W_encT.device)
+        vals = d_vals.to(self.dtype)
+        bias = torch.zeros(self.A_s, dtype=self.dtype, device=W_encT.device)
+        check(self.lib.mtc_decode_fwd(C.byref(d), _p(sel.row_ptr), _p(sel.col_idx), _p(vals), _p(W_encT), _p(bias), None, None, None,
+                                      _p(dx), None, None, None, None, 0.0, _stream()), "mtc_decode_fwd")
+        return dx
+
     def decode_bwd_vals(self, d, sel: Selection, W_dec, g, l1_term: float):
         d_vals = torch.empty(sel.col_idx.numel(), dtype=torch.float32, device=g.device)
         check(self.lib.mtc_decode_bwd_vals(C.byref(d), _p(sel.row_ptr), _p(sel.col_idx), _p(W_dec), _p(g), float(l1_term),

@@ -689,6 +689,10 @@ class ShardedMatryoshkaTranscoder(MatryoshkaTranscoder):
     def gathered_dead_counters(self) -> torch.Tensor:
         return self._gather_features(self._cnt, 0)
 
+    def reconstruct(self, x_source):
+        raise _lib.MtcError("reconstruct() runs on the single-GPU model only: the sharded one offers encode() / decode() without "
+                            "gradient")
+
     def encode(self, x_source):
         """Dense [.., D] features in GLOBAL feature order (collective)."""
         shape = x_source.shape

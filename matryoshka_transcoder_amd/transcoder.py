@@ -62,6 +62,39 @@ class _StepFn(torch.autograd.Function):
         return None, None, None, dW_encT.t(), db_enc, dW_dec, db_dec
 
 
+class _ReconstructFn(torch.autograd.Function):
+    """Standardised input -> selected features -> reconstruction, for any incoming gradient (the training step's own backward,
+    _StepFn, starts from its loss).  Gradients flow through the selected features only, as in sae.py:173-191."""
+
+    @staticmethod
+    def forward(ctx, module, x, W_enc, b_enc, W_dec, b_dec, mean, std):
+        hp = module.hot_path()
+        d = hp.desc(x.shape[0])
+        acts = hp.encode(d, x, module._w_encT(W_enc), b_enc.contiguous())
+        sel = module._select(hp, d, acts, module.training)
+        ctx.module, ctx.sel = module, sel
+        ctx.save_for_backward(x, W_enc, W_dec)
+        return hp.reconstruct(sel, W_dec.contiguous(), b_dec.contiguous(), x.shape[0], mean, std)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        module, sel = ctx.module, ctx.sel
+        x, W_enc, W_dec = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[1], any(ctx.needs_input_grad[2:6])
+        with module._on_device():
+            hp = module.hot_path()
+            d = hp.desc(x.shape[0])
+            g = g.contiguous()
+            d_vals = hp.decode_bwd_vals(d, sel, W_dec.contiguous(), g, 0.0)
+            dx = hp.encoder_input_grad(sel, d_vals, module._w_encT(W_enc), x.shape[0]) if need_x else None
+            if not need_w:
+                return None, dx, None, None, None, None, None, None
+            hp.build_csc(d, sel, None)
+            dW_dec, dW_encT, db_enc, db_dec = hp.backward(d, sel, g, d_vals, x, None)
+        return None, dx, dW_encT.t(), db_enc, dW_dec, db_dec, None, None
+
+
 class MatryoshkaTranscoder(nn.Module):
     """Cross-layer transcoder with nested (Matryoshka) prefix groups and global batch-TopK sparsity."""
 
@@ -500,6 +533,40 @@ class MatryoshkaTranscoder(nn.Module):
             "fvu_max": s[8],
             "fvu_mean": s[9],
         }
+
+    def reconstruct(self, x_source):
+        """`decode(encode(x_source))` (sae.py:363-406) without the dense feature tensor, differentiable in x_source and the
+        parameters: what a model's block needs when the transcoder stands in for its MLP (splice.py).  Any leading shape;
+        honours train / eval mode as `encode` does (in train mode the global TopK moves the threshold's average; the dead
+        counters stay).  Statistics of the input standardisation are kept like `encode`'s and take part in the gradient."""
+        self._check_inputs(x_source)
+        if x_source.shape[-1] != self.source_act_size:
+            raise _lib.MtcError(f"reconstruct() needs activations of width {self.source_act_size}, got {list(x_source.shape)}")
+        if self.prefix_indices[self.active_prefixes] != self.total_dict_size:
+            raise _lib.MtcError("reconstruct() runs the whole dictionary: use encode() / decode() with active_prefixes")
+        lead = x_source.shape[:-1]
+        x = x_source.reshape(-1, self.source_act_size).contiguous()
+        if x.shape[0] == 0:
+            return x_source.new_empty(lead + (self.target_act_size,))
+        params = (self.W_enc, self.b_enc, self.W_dec, self.b_dec)
+        unit = bool(self.config.get("input_unit_norm", False))
+        with self._on_device():
+            if not unit:
+                self.x_mean = self.x_std = None
+                return _ReconstructFn.apply(self, x, *params, None, None).reshape(lead + (-1,))
+            if not (torch.is_grad_enabled() and x.requires_grad):
+                xn, self.x_mean, self.x_std = self.preprocess_input(x)
+                if not (torch.is_grad_enabled() and any(p.requires_grad for p in params)):
+                    return _ReconstructFn.apply(self, xn, *params, self.x_mean.reshape(-1), self.x_std.reshape(-1)).reshape(lead + (-1,))
+                mean, std = self.x_mean, self.x_std
+            else:
+                # the reference's own steps (sae.py:139-147), each an autograd op: mean and deviation carry gradient to x
+                mean = x.mean(dim=-1, keepdim=True)
+                xc = x - mean
+                std = xc.std(dim=-1, keepdim=True)
+                xn = xc / (std + 1e-5)
+                self.x_mean, self.x_std = mean.detach(), std.detach()
+            return self.postprocess_output(_ReconstructFn.apply(self, xn, *params, None, None), mean, std).reshape(lead + (-1,))
 
     def encode(self, x_source):
         """sae.py:363-387: dense sparse-feature tensor, 2-D or 3-D input; honours train/eval mode."""
