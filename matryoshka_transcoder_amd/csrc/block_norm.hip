@@ -14,6 +14,7 @@
 // workgroup holds `groups` such row groups.  Row sums: DPP inside a wave, one LDS exchange across the row's waves.
 // Rows whose width is a multiple of 8 with 16-byte-aligned rows use 16-byte accesses (columns 8 t .. 8 t + 7); any other
 // width or stride takes the same kernel with single elements (columns t, t + T, ..., which keeps a wave's accesses side by side).
+#include <algorithm>
 #include <type_traits>
 #include "common.hpp"
 
@@ -30,7 +31,7 @@ struct NormRow {                         // one row-major operand: base, row str
 struct NormArgs {
     long long rows;
     int A, T, groups;
-    int post_kind, pre_kind, gate_kind;
+    int post_kind, pre_kind, gate_kind, streaming;
     float post_eps, pre_eps, post_off, pre_off, res_scale, branch_scale, inv_A;
     NormRow residual, branch, gate, hidden, normed;
     const void *post_w, *post_b, *pre_w, *pre_b;
@@ -314,6 +315,165 @@ __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
     });
 }
 
+// Forward with one wave per row, where its registers hold the row: no barriers, the row sums stay inside the wave, and what a
+// row costs besides its elements (addresses, reductions) is paid once per row instead of once per wave and row.  A lane holds
+// NU units of 16 bytes, the wave's accesses are contiguous.  Every row is a wave of its own, dispatched in order, so that the
+// rows in flight are neighbours in memory.  Against the row group kernel above: 65536 x 2304 bf16 norm alone 97 against
+// 108 us (6.2 TB/s), 32768 x 2304 pair 98 against 115, 16384 x 2304 fp32 pair 100 against 112, 4096 x 2304 bf16 pair called in
+// a row 12.3 against 13.3.
+//   PLAIN: no bias and no gate per channel or element, which saves the registers of two rows.
+template <int DT, int NU> struct WaveRow {
+    static constexpr int E = DType<DT>::kVec;
+    u32x4 r[NU];
+    __device__ __forceinline__ void load(rsrc_t s, int lane, bool streaming) {
+        if (streaming) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(s, (u * 64 + lane) * 16, 0, 2);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(s, (u * 64 + lane) * 16, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void unpack(int u, float (&v)[E]) const {
+        if constexpr (DT == MTC_BF16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(r[u][i] << 16);
+                v[2 * i + 1] = __uint_as_float(r[u][i] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[u][i]);
+        }
+    }
+    __device__ __forceinline__ void pack(int u, const float (&v)[E]) {
+        if constexpr (DT == MTC_BF16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[u][i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[u][i] = __float_as_uint(v[i]);
+        }
+    }
+    __device__ __forceinline__ void store(rsrc_t s, int lane, bool streaming) const {
+        if (streaming) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) __builtin_amdgcn_raw_buffer_store_b128(r[u], s, (u * 64 + lane) * 16, 0, 2);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) __builtin_amdgcn_raw_buffer_store_b128(r[u], s, (u * 64 + lane) * 16, 0, 0);
+        }
+    }
+};
+// v becomes v - mean (layer); returns 1/std
+template <int NU, int E>
+__device__ __forceinline__ float wave_normalise(float (&v)[NU][E], int kind, float eps, float inv_A, int lane, int A, float& mu) {
+    mu = 0.f;
+    if (kind == MTC_NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int i = 0; i < E; ++i) s += v[u][i];
+        mu = wave_total(s) * inv_A;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const float m = (u * 64 + lane) * E < A ? mu : 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[u][i] -= m;
+        }
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int i = 0; i < E; ++i) q = fmaf(v[u][i], v[u][i], q);
+    return 1.f / sqrtf(fmaf(wave_total(q), inv_A, eps));
+}
+
+template <int DT, int NU, bool BRANCH, bool PRE, bool PLAIN>
+__global__ __launch_bounds__(256, (BRANCH && NU <= 5 ? 4 : 1)) void block_norm_wave_kernel(NormArgs a) {
+    constexpr int E = DType<DT>::kVec, ES = (int)sizeof(typename DType<DT>::T);
+    typedef WaveRow<DT, NU> Row;
+    const int lane = threadIdx.x & 63;
+    const long long row = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) + (long long)blockIdx.x * (blockDim.x >> 6);
+    if (row >= a.rows) return;
+    const int bytes = a.A * ES;
+    const bool nt = a.streaming;
+    auto rsrc = [&](const NormRow& o) { return rows_rsrc(o.p, row * o.ld * ES, bytes); };
+    auto vec = [&](const void* p) { return rows_rsrc(p, 0, bytes); };
+    Row r, y, g, w, b;
+    r.load(rsrc(a.residual), lane, nt);
+    if (BRANCH) y.load(rsrc(a.branch), lane, nt);
+    float h[NU][E], t[E], st[4] = {0.f, 0.f, 0.f, 0.f};
+    // h <- (h * rstd) * (offset + weight) + bias
+    auto affine = [&](bool has_w, float off, bool has_b, float rstd) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            if (has_w) {
+                w.unpack(u, t);
+#pragma unroll
+                for (int i = 0; i < E; ++i) h[u][i] *= rstd * (off + t[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) h[u][i] *= rstd;
+            }
+            if (has_b) {
+                b.unpack(u, t);
+#pragma unroll
+                for (int i = 0; i < E; ++i) h[u][i] += t[i];
+            }
+        }
+    };
+    if (BRANCH) {
+        const bool post = a.post_kind != MTC_NORM_NONE, has_w = post && a.post_w, has_b = !PLAIN && post && a.post_b;
+        const bool chan = !PLAIN && a.gate_kind == MTC_GATE_CHANNEL, full = !PLAIN && a.gate_kind == MTC_GATE_FULL;
+        if (has_w) w.load(vec(a.post_w), lane, false);
+        if (has_b) b.load(vec(a.post_b), lane, false);
+        if (chan) g.load(vec(a.gate.p), lane, false);
+        if (full) g.load(rsrc(a.gate), lane, nt);
+        float scale = a.branch_scale;
+        if (a.gate_kind == MTC_GATE_ROW || a.gate_kind == MTC_GATE_SCALAR)
+            scale *= __uint_as_float(fetch_one<DT>(a.gate, row, true));
+#pragma unroll
+        for (int u = 0; u < NU; ++u) y.unpack(u, h[u]);
+        if (post) {
+            st[1] = wave_normalise<NU, E>(h, a.post_kind, a.post_eps, a.inv_A, lane, a.A, st[0]);
+            affine(has_w, a.post_off, has_b, st[1]);
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            if (chan || full) {
+                g.unpack(u, t);
+#pragma unroll
+                for (int i = 0; i < E; ++i) h[u][i] *= t[i];
+            }
+            r.unpack(u, t);
+#pragma unroll
+            for (int i = 0; i < E; ++i) h[u][i] = fmaf(scale, h[u][i], a.res_scale * t[i]);
+            r.pack(u, h[u]);
+        }
+        r.store(rsrc(a.hidden), lane, nt);
+    } else {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) r.unpack(u, h[u]);
+    }
+    if (PRE) {
+        const bool has_w = a.pre_w, has_b = !PLAIN && a.pre_b;
+        if (has_w) w.load(vec(a.pre_w), lane, false);
+        if (has_b) b.load(vec(a.pre_b), lane, false);
+        st[3] = wave_normalise<NU, E>(h, a.pre_kind, a.pre_eps, a.inv_A, lane, a.A, st[2]);
+        affine(has_w, a.pre_off, has_b, st[3]);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) y.pack(u, h[u]);
+        y.store(rsrc(a.normed), lane, nt);
+    }
+    if (a.stats && lane == 0) {
+        const u32x4 v = {__float_as_uint(st[0]), __float_as_uint(st[1]), __float_as_uint(st[2]), __float_as_uint(st[3])};
+        *reinterpret_cast<u32x4*>(a.stats + row * 4) = v;
+    }
+}
+
 // Gradient.  With g = d_normed, du = g (offset + w_pre):
 //     D        = d_hidden + rstd (du - [layer] mean(du) - u mean(du u))          d_residual = residual_scale D
 //     dv       = D gate pf                                                       (pf: branch scale x channel gate x post weight)
@@ -585,6 +745,7 @@ static int norm_check(const mtc_block_norm_desc* d, const char* who) {
 static int norm_threads(int A) { return ((A + 7) / 8 + 63) / 64 * 64; }
 
 constexpr int NORM_BWD_T = 768;                    // threads of a backward workgroup, if a row needs no more: 168 registers each
+constexpr long long WAVE_MAX_ROWS = 1ll << 25;             // one wave each: a launch has at most 2^32 threads
 constexpr long long NORM_STREAM_BYTES = 256ll << 20;       // the Infinity Cache
 
 // workgroups for `want` row sets: at most per_cu on each CU, and every one the same number of rounds
@@ -640,9 +801,46 @@ template <int DT, bool VEC, bool STREAM> static void launch_norm_fwd(const NormA
     else hipLaunchKernelGGL((block_norm_fwd_kernel<DT, VEC, true, false, false, STREAM>), g, b, 0, s, a);
 }
 
-template <int DT> static void launch_norm_fwd_dt(const NormArgs& a, bool branch, bool vec, bool stream, unsigned grid, hipStream_t s) {
+// What a wave can hold: 9 units a lane for a norm alone; with a branch 40 floats of a row, 36 where biases or a gate per
+// channel or element need rows of their own.  Beyond, the row group kernel is faster (4096 x 4608 bf16 pair 30 against
+// 47 us, 16384 x 2304 bf16 layer norms with a channel gate 65 against 78).
+template <int DT, bool BRANCH, bool PLAIN> constexpr int wave_units() {
+    return !BRANCH ? 9 : std::min(9, (PLAIN ? 40 : 36) / DType<DT>::kVec);
+}
+
+template <int DT, int NU, bool PLAIN> static bool launch_norm_wave(const NormArgs& a, bool branch, hipStream_t s) {
+    const int per = a.rows < 4 * NORM_CUS ? 1 : 4;
+    const dim3 g((unsigned)((a.rows + per - 1) / per)), b(64 * per);
+    if (!branch) {
+        hipLaunchKernelGGL((block_norm_wave_kernel<DT, NU, false, true, PLAIN>), g, b, 0, s, a);
+        return true;
+    }
+    if constexpr (NU <= wave_units<DT, true, PLAIN>()) {
+        if (a.pre_kind != MTC_NORM_NONE) hipLaunchKernelGGL((block_norm_wave_kernel<DT, NU, true, true, PLAIN>), g, b, 0, s, a);
+        else hipLaunchKernelGGL((block_norm_wave_kernel<DT, NU, true, false, PLAIN>), g, b, 0, s, a);
+        return true;
+    }
+    return false;
+}
+
+template <int DT, bool PLAIN> static bool launch_norm_wave_units(const NormArgs& a, bool branch, hipStream_t s) {
+    switch ((a.A * norm_elem(DT) + 1023) / 1024) {
+        case 1: return launch_norm_wave<DT, 1, PLAIN>(a, branch, s);
+        case 2: return launch_norm_wave<DT, 2, PLAIN>(a, branch, s);
+        case 3: return launch_norm_wave<DT, 3, PLAIN>(a, branch, s);
+        case 4: case 5: return launch_norm_wave<DT, 5, PLAIN>(a, branch, s);
+        case 6: case 7: return launch_norm_wave<DT, 7, PLAIN>(a, branch, s);
+        case 8: case 9: return launch_norm_wave<DT, 9, PLAIN>(a, branch, s);
+        default: return false;
+    }
+}
+
+template <int DT> static void launch_norm_fwd_dt(const NormArgs& a, bool branch, bool vec, unsigned grid, hipStream_t s) {
+    const bool plain = !a.post_b && !a.pre_b && a.gate_kind != MTC_GATE_CHANNEL && a.gate_kind != MTC_GATE_FULL;
+    if (vec && a.rows <= WAVE_MAX_ROWS && (plain ? launch_norm_wave_units<DT, true>(a, branch, s) : launch_norm_wave_units<DT, false>(a, branch, s)))
+        return;
     if (!vec) launch_norm_fwd<DT, false, false>(a, branch, grid, s);
-    else if (stream) launch_norm_fwd<DT, true, true>(a, branch, grid, s);
+    else if (a.streaming) launch_norm_fwd<DT, true, true>(a, branch, grid, s);
     else launch_norm_fwd<DT, true, false>(a, branch, grid, s);
 }
 
@@ -668,17 +866,17 @@ extern "C" int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* resi
                      row_vec(normed, d->ld_normed, d->rows, d->dtype);
     a.groups = a.T >= 256 ? 1 : 256 / a.T;
     // operands read and written once; beyond the Infinity Cache non-temporal accesses and, for two RMS norms (whose rows wait
-    // least), few waves that keep to few DRAM pages are faster: 16384 x 4608 bf16 pair 99 against 118 us, 65536 x 2304
-    // norm alone 109 against 115.  Within the cache the opposite holds: 4096 x 2304 pair 14.8 against 17.0 us, and what
-    // follows finds plain stores in the cache (four such calls in a row 60 against 65 us).
+    // least), few waves that keep to few DRAM pages are faster: 16384 x 4608 bf16 pair 99 against 118 us.  Within the cache the
+    // opposite holds: 4096 x 2304 pair 14.8 against 17.0 us, and what follows finds plain stores in the cache (four such
+    // calls in a row 60 against 65 us).
     const int passes = (branch ? 2 : 1) + (d->gate_kind == MTC_GATE_FULL) + (hidden != nullptr) + (normed != nullptr);
-    const bool streaming = d->rows * d->A * norm_elem(d->dtype) * passes > NORM_STREAM_BYTES;
+    a.streaming = d->rows * d->A * norm_elem(d->dtype) * passes > NORM_STREAM_BYTES;
     const bool layer = d->post_kind == MTC_NORM_LAYER || d->pre_kind == MTC_NORM_LAYER;
-    const int waves = !streaming ? 20 : branch && !layer ? 12 : 28;
+    const int waves = !a.streaming ? 20 : branch && !layer ? 12 : 28;
     const unsigned grid = norm_grid((d->rows + a.groups - 1) / a.groups, waves / (a.T * a.groups / 64));
     hipStream_t s = as_stream(stream);
-    if (d->dtype == MTC_BF16) launch_norm_fwd_dt<MTC_BF16>(a, branch, vec, streaming, grid, s);
-    else launch_norm_fwd_dt<MTC_F32>(a, branch, vec, streaming, grid, s);
+    if (d->dtype == MTC_BF16) launch_norm_fwd_dt<MTC_BF16>(a, branch, vec, grid, s);
+    else launch_norm_fwd_dt<MTC_F32>(a, branch, vec, grid, s);
     return check_launch(who);
 }
 

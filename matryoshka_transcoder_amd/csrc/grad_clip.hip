@@ -25,6 +25,7 @@ constexpr int CLIP_BATCH = 128;            // tensors per launch (kernel argumen
 constexpr int TILE_UNITS = 1024;           // 16-byte units per tile: 4 per thread
 constexpr int PER_THREAD = TILE_UNITS / 256;
 constexpr int CLIP_GRID = 2048;            // workgroups of one launch that walk over tiles
+constexpr int LARGE_GRID = 1 << 22;        // a workgroup per tile up to 64 GiB (a launch has at most 2^32 threads)
 constexpr int SMALL_TILES = 8192;          // 128 MiB
 constexpr uint64_t STREAM_TILES = 32768;   // 512 MiB: twice the Infinity Cache
 constexpr float CLIP_EPS = 1e-6f;
@@ -399,9 +400,9 @@ template <int POW> static void clip_launch(const ClipList& l, double* ws, float 
                                norm_out);
             norm_out = nullptr;                          // the first launch has written it
         } else if (streaming) {
-            hipLaunchKernelGGL(clip_large_kernel<true>, dim3(b.tiles), dim3(256), 0, s, b, norm_coef, in_place);
+            hipLaunchKernelGGL(clip_large_kernel<true>, dim3(std::min(b.tiles, LARGE_GRID)), dim3(256), 0, s, b, norm_coef, in_place);
         } else {
-            hipLaunchKernelGGL(clip_large_kernel<false>, dim3(b.tiles), dim3(256), 0, s, b, norm_coef, in_place);
+            hipLaunchKernelGGL(clip_large_kernel<false>, dim3(std::min(b.tiles, LARGE_GRID)), dim3(256), 0, s, b, norm_coef, in_place);
         }
     }
 }

@@ -83,14 +83,14 @@ def _check(rows, A, dt, mode, post_kind, pre_kind, gate_kind, rs=1.0, bs=1.0, se
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("rows,A", [(1, 2304), (3, 768), (130, 1600), (257, 2304), (65, 4608), (9, 8192), (1, 8), (70, 64),
+@pytest.mark.parametrize("rows,A", [(1030, 1024), (1025, 3584), (9, 1536), (1, 2304), (3, 768), (130, 1600), (257, 2304), (65, 4608), (9, 8192), (1, 8), (70, 64),
                                     (33, 520), (1, 1), (5, 7), (300, 1001), (2, 8191)])
 def test_pair_rms(rows, A, dt):
     _check(rows, A, dt, "pair", "rms", "rms", "none")
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("rows,A", [(1, 768), (131, 1600), (17, 1283), (40, 4608)])
+@pytest.mark.parametrize("rows,A", [(1, 768), (131, 1600), (17, 1283), (40, 4608), (30, 256), (29, 1280), (5, 2304)])
 @pytest.mark.parametrize("gate", ["none", "scalar", "token", "channel", "full"])
 def test_pair_layer_gates(rows, A, gate, dt):
     _check(rows, A, dt, "pair", "layer", "layer", gate, rs=0.75, bs=1.5)
@@ -256,6 +256,28 @@ def test_streaming_sizes(dt):
     N.compare("post_w", whole[4], N.reference(res, br, None, _spec(post), _spec(pre), 1.0, 1.0, dh, dn)["post_w"], dt)
     alone = block_norm(res, pre.weight, eps=1e-6, weight_offset=1.0)
     assert torch.equal(alone[1000:2000], block_norm(res[1000:2000], pre.weight, eps=1e-6, weight_offset=1.0))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements, and more rows than one launch has waves for: the far rows equal a call on them alone."""
+    for rows, A in (((1 << 31) // 2304 + 1000, 2304), ((1 << 25) + 77, 8)):
+        x = torch.zeros(rows, A, dtype=torch.bfloat16, device=DEV)
+        gen = torch.Generator(DEV).manual_seed(19)
+        x[-300:] = torch.randn(300, A, generator=gen, device=DEV).bfloat16()
+        m = BlockNorm(A, kind="layer", dtype=torch.bfloat16, device=DEV)
+        with torch.no_grad():
+            y = m(x)
+            assert torch.equal(y[-300:], m(x[-300:])) and not bool(y[:1000].any())
+            h, n = residual_block_norm(x, x, m, pre=m)
+            h2, n2 = residual_block_norm(x[-300:], x[-300:], m, pre=m)
+            assert torch.equal(h[-300:], h2) and torch.equal(n[-300:], n2)
+        del y, h, n
+        r = x.requires_grad_(True)
+        (g,) = torch.autograd.grad(m(r), [r], x.detach())
+        r2 = x[-300:].detach().requires_grad_(True)
+        (g2,) = torch.autograd.grad(m(r2), [r2], r2.detach())
+        assert torch.equal(g[-300:], g2)
+        del x, r, g
 
 
 def test_gradient_against_differences():
