@@ -326,8 +326,10 @@ Tensor clip(const std::vector<Tensor>& src, const std::optional<std::vector<Tens
     check(lib.grad_clip((int32_t)a.size(), call.src.data(), to.data(), call.elems.data(), call.dtype.data(), p, limit, call.ws.data_ptr(),
                         call.ws_bytes, norm.data_ptr<float>(), stream_of(norm)),
           "mtc_grad_clip");
-    for (size_t i = 0; i < src.size(); ++i)
+    for (size_t i = 0; i < src.size(); ++i) {
         if (back[i].defined()) dst[i].copy_(back[i]);
+        else if (!dst[i].is_inference()) dst[i].unsafeGetTensorImpl()->bump_version();       // written behind autograd's back
+    }
     return norm;
 }
 

@@ -30,12 +30,12 @@ def _list(tensors: Tensors) -> List[torch.Tensor]:
 
 def norm_and_coef(tensors: Tensors, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """float32 [2] on the GPU: the norm and the factor that clips to max_norm."""
-    return _lib.torch_binding().norm_of(_list(tensors), norm_type, max_norm, False)
+    return _lib.torch_binding().norm_of(_list(tensors), float(norm_type), float(max_norm), False)
 
 
 def power_sum(tensors: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     """float64 scalar on the GPU: the norm's sum before its root (p = inf: the maximum), to be combined over ranks."""
-    return _lib.torch_binding().norm_of(_list(tensors), norm_type, math.inf, True)
+    return _lib.torch_binding().norm_of(_list(tensors), float(norm_type), math.inf, True)
 
 
 def coef_of_power_sum(total: torch.Tensor, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
@@ -66,7 +66,7 @@ def clip_by_global_norm_(tensors: Tensors, max_norm: float, norm_type: float = 2
     src = _list(tensors)
     if error_if_nonfinite and src and not math.isfinite(float(global_norm(src, norm_type))):
         raise RuntimeError(f"the total norm of order {norm_type} of the gradients is non-finite, so it cannot be clipped")
-    return _lib.torch_binding().clip(src, None if out is None else _list(out), norm_type, max_norm)
+    return _lib.torch_binding().clip(src, None if out is None else _list(out), float(norm_type), float(max_norm))
 
 
 def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:

@@ -210,6 +210,15 @@ def test_captured_and_replayed():
         assert torch.equal(norm, want) and all(torch.equal(t, x) for t, x in zip(ts, new))
 
 
+def test_clipping_a_saved_tensor_is_noticed():
+    """A tensor that autograd saved and that is clipped afterwards: its version moves, so the backward refuses."""
+    a, b = torch.ones(8, device=DEV, requires_grad=True), torch.full((8,), 2.0, device=DEV)
+    c = (a * b).sum()
+    clip_by_global_norm_([b], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        c.backward()
+
+
 def test_parameters():
     ps = [torch.nn.Parameter(torch.randn(100, device=DEV)) for _ in range(3)]
     ps[0].grad, ps[2].grad = torch.randn(100, device=DEV), torch.randn(100, device=DEV)
