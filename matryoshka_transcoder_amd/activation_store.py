@@ -22,6 +22,7 @@ from typing import Iterator, Optional, Tuple
 
 import torch
 
+from . import _lib
 from .config import create_transcoder_config  # noqa: F401  (re-exported like the reference module)
 
 
@@ -68,6 +69,8 @@ class TranscoderActivationsStore:
         harvest or store instead of two, for models that have no hook behind that norm."""
         self.model = model
         self.source_norm = cfg.get("source_norm")
+        if self.source_norm is not None and not isinstance(self.source_norm, torch.nn.Module):
+            raise _lib.MtcError(f"cfg['source_norm'] must be a module such as BlockNorm, got {self.source_norm!r}")
         self.config = cfg
         self.device = cfg["device"]
         self.source_hook_point = cfg.get("source_hook_point")
@@ -163,7 +166,6 @@ class TranscoderActivationsStore:
             # bookkeeping (buffer refill, permutation, short last batch, aligned pairs) through this branch
             return src.index_select(0, idx), tgt.index_select(0, idx)
         import ctypes as C
-        from . import _lib
         from .engine import _p, _stream, dtype_code
         if not (src.is_contiguous() and tgt.is_contiguous() and src.dtype == tgt.dtype and tgt.device == src.device):
             raise _lib.MtcError("activation buffers must be contiguous, of one dtype, on one GPU")

@@ -21,12 +21,12 @@ import torch
 
 
 def _jsonable(obj: Any) -> Any:
-    """dtype / device objects become their string form; containers are walked."""
+    """dtype / device objects and modules (cfg["source_norm"]) become their string form; containers are walked."""
     if isinstance(obj, dict):
         return {key: _jsonable(val) for key, val in obj.items()}
     if isinstance(obj, (tuple, list)):
         return [_jsonable(val) for val in obj]
-    return str(obj) if isinstance(obj, (torch.device, torch.dtype)) else obj
+    return str(obj) if isinstance(obj, (torch.device, torch.dtype, torch.nn.Module)) else obj
 
 
 def _dump(path: Path, payload: Any) -> None:

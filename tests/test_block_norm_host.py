@@ -1,5 +1,6 @@
 """What the block norms refuse before any launch (no GPU needed)."""
 import ctypes as C
+import json
 
 import pytest
 import torch
@@ -81,3 +82,17 @@ def test_module_parameters():
     m = BlockNorm(64, kind="layer")
     assert list(m.state_dict()) == ["weight", "bias"] and bool((m.weight == 1).all()) and not bool(m.bias.any())
     assert list(BlockNorm(64, affine=False).state_dict()) == []
+
+
+def test_a_run_with_a_source_norm_can_be_saved(tmp_path):
+    """The configuration of a run is written as JSON with every checkpoint: a module in it appears by its description."""
+    from matryoshka_transcoder_amd.activation_store import TranscoderActivationsStore
+    from matryoshka_transcoder_amd.results import CleanResultsManager
+    results = CleanResultsManager(str(tmp_path))
+    run = results.create_experiment_dir("m", 0, 1)
+    cfg = {"dtype": torch.bfloat16, "act_size": 64, "device": "cpu", "source_norm": BlockNorm(64)}
+    results.save_checkpoint(run, torch.nn.Linear(2, 2), cfg, 1)
+    saved = json.loads((run / "config.json").read_text())
+    assert saved["source_norm"].startswith("BlockNorm(64, kind='rms'")
+    with pytest.raises(_lib.MtcError, match="source_norm"):                 # what was saved is no module any more
+        TranscoderActivationsStore(None, dict(cfg, source_norm=saved["source_norm"]))
