@@ -5,10 +5,13 @@
 // points are handed over by address (bind), so that this module and ctypes drive the one library that is loaded.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <limits>
 #include <sstream>
 #include <string>
@@ -123,6 +126,17 @@ std::tuple<Tensor, Tensor> norm_forward(const Plan& p, const Tensor& residual, c
 
 Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+// The engine adds a leaf's gradient on the stream on which the leaf's accumulation node was made, and an eager graph that is still alive
+// keeps that node.  Recorded into a HIP graph, the default stream would have to wait for the recording, which ends the process.
+void check_recorded_leaf(const Tensor& t) {
+    if (!t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && stream->id() == 0)
+        fail("a backward of the block norms cannot be recorded into a HIP graph while an eager graph of the same leaf, made on the default "
+             "stream, is alive: release it first (its outputs or loss)");
+}
+
 struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& residual, const OptTensor& branch, const OptTensor& gate,
                                  const OptTensor& post_w, const OptTensor& post_b, const OptTensor& pre_w, const OptTensor& pre_b, const Plan& p) {
@@ -146,8 +160,13 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
         if (!dh.defined() && !dn.defined()) return out;
         const bool pre = dn.defined();
         c10::DeviceGuard guard(residual.device());
-        for (int i = 0; i < 7; ++i) {
-            if (!p.need[i]) continue;
+        const bool recording = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+        bool need[7];
+        for (int i = 0, edge = 0; i < 7; ++i) {
+            need[i] = p.need[i] && ctx->needs_input_grad(edge);      // edges: the operands that are there
+            edge += s[1 + i].defined();
+            if (!need[i]) continue;
+            if (recording) check_recorded_leaf(s[1 + i]);
             // rows of nothing, and a pre norm whose output nobody used, leave zeros
             const bool zero = !p.rows || (i >= 5 && !pre);
             out[i] = zero ? at::zeros(s[1 + i].sizes(), residual.options()) : at::empty(s[1 + i].sizes(), residual.options());
@@ -160,8 +179,8 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
         if (pre) dn = rows_of(dn, p.A, ld_dn);
         Tensor ws;
         size_t ws_bytes = 0;
-        const bool gate_sum = p.need[2] && (p.gate_kind == MTC_GATE_CHANNEL || p.gate_kind == MTC_GATE_SCALAR);
-        if (p.need[3] || p.need[4] || p.need[5] || p.need[6] || gate_sum) {
+        const bool gate_sum = need[2] && (p.gate_kind == MTC_GATE_CHANNEL || p.gate_kind == MTC_GATE_SCALAR);
+        if (need[3] || need[4] || need[5] || need[6] || gate_sum) {
             ws_bytes = lib.norm_ws(&d);
             ws = at::empty({(int64_t)ws_bytes}, residual.options().dtype(at::kByte));
         }
@@ -218,6 +237,8 @@ std::tuple<OptTensor, OptTensor> block_norm(const Tensor& residual, const OptTen
                             norm_vector(post_b, p.A, residual, "post", "bias"), norm_vector(pre_w, p.A, residual, "pre", "weight"),
                             norm_vector(pre_b, p.A, residual, "pre", "bias")};
     p.gate_kind = gate_kind(gate, residual);
+    for (const OptTensor& x : t)
+        if (x.has_value() && x->defined() && x->_fw_grad(0).defined()) fail("the block norms have no forward-mode derivative");
     bool any = false;
     if (at::GradMode::is_enabled())
         for (int i = 0; i < 7; ++i) any |= p.need[i] = t[i].has_value() && t[i]->defined() && t[i]->requires_grad();
@@ -295,6 +316,28 @@ Tensor norm_of(const std::vector<Tensor>& ts, double order, double max_norm, boo
     return out;
 }
 
+// mtc_grad_clip refuses outputs that share memory; those written by a copy after it are held to the same, by the ranges they span
+void check_copied_outputs(const std::vector<Tensor>& dst, const std::vector<Tensor>& copied) {
+    struct Span { uintptr_t a, b; size_t i; };
+    std::vector<Span> s;
+    bool any = false;
+    for (size_t i = 0; i < dst.size(); ++i) {
+        if (!dst[i].numel()) continue;
+        uintptr_t elems = 1;
+        for (int64_t k = 0; k < dst[i].dim(); ++k) elems += (uintptr_t)((dst[i].size(k) - 1) * dst[i].stride(k));
+        const uintptr_t a = (uintptr_t)dst[i].data_ptr();
+        s.push_back({a, a + elems * dst[i].element_size(), i});
+        any |= copied[i].defined();
+    }
+    if (!any) return;
+    std::sort(s.begin(), s.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    for (size_t k = 1, last = 0; k < s.size(); ++k) {                // last: the furthest end so far
+        if (s[k].a < s[last].b && (copied[s[k].i].defined() || copied[s[last].i].defined()))
+            fail("outputs ", s[last].i, " and ", s[k].i, " span the same memory");
+        if (s[k].b > s[last].b) last = k;
+    }
+}
+
 Tensor clip(const std::vector<Tensor>& src, const std::optional<std::vector<Tensor>>& out, double order, double max_norm) {
     const float p = norm_order(order), limit = norm_limit(max_norm);
     const std::vector<Tensor>& dst = out.has_value() ? *out : src;
@@ -321,6 +364,7 @@ Tensor clip(const std::vector<Tensor>& src, const std::optional<std::vector<Tens
         if (a[i].numel() && dst[i].strides() != a[i].strides()) back[i] = at::empty_like(a[i]);
         to[i] = !a[i].numel() ? nullptr : back[i].defined() ? back[i].data_ptr() : dst[i].data_ptr();
     }
+    if (out.has_value()) check_copied_outputs(dst, back);
     const ClipCall call(a);
     const Tensor norm = at::empty({}, src[0].options().dtype(at::kFloat));
     check(lib.grad_clip((int32_t)a.size(), call.src.data(), to.data(), call.elems.data(), call.dtype.data(), p, limit, call.ws.data_ptr(),

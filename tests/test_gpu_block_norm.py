@@ -420,3 +420,60 @@ def test_refusals_on_the_gpu():
         r = x.clone().requires_grad_(True)
         (gr,) = torch.autograd.grad(block_norm(r).sum(), [r], create_graph=True)
         gr.sum().backward()
+
+
+def test_recording_beside_a_live_eager_graph_is_refused():
+    """The refusal comes before the engine touches the leaf's accumulation node; once the eager graph is gone, the same
+    recording works."""
+    x = torch.randn(7, 128, device=DEV).requires_grad_(True)
+    norm = BlockNorm(128, device=DEV)
+    d = torch.randn(7, 128, device=DEV)
+    alive = norm(x)                                                  # keeps the leaves' nodes of the default stream
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(norm(x), [x, norm.weight], d)
+    with torch.no_grad():
+        want = block_norm(x, norm.weight)
+    assert torch.equal(alive, want)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(norm(x), [x, norm.weight], d)
+    for _ in range(2):
+        with torch.no_grad():
+            x.copy_(torch.randn(7, 128, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        y = x.detach().clone().requires_grad_(True)
+        for a, b in zip(got, torch.autograd.grad(norm(y), [y, norm.weight], d)):
+            assert torch.equal(a, b)
+
+
+def test_only_the_asked_gradients_are_computed():
+    """autograd.grad over a part of the leaves: the same bits as with all of them."""
+    g = torch.Generator("cpu").manual_seed(23)
+    post, pre = _norm_module(g, 96, "layer", torch.float32), _norm_module(g, 96, "rms", torch.float32)
+    r, b, gate = (_rand(g, *s).to(DEV).requires_grad_(True) for s in ((9, 96), (9, 96), (9, 1)))
+    leaves = [r, b, gate, post.weight, post.bias, pre.weight]
+    d = _rand(g, 9, 96).to(DEV)
+    grads = lambda which: torch.autograd.grad(residual_block_norm(r, b, post, gate=gate, pre=pre), which, [d, d])      # noqa: E731
+    for leaf, want in zip(leaves, grads(leaves)):
+        assert torch.equal(grads([leaf])[0], want)
+    for leaf in leaves[:3]:                                          # without a gate the edges behind it move up
+        if leaf is not gate:
+            assert torch.autograd.grad(residual_block_norm(r, b, post), [leaf], d)[0].shape == leaf.shape
+    (dw,) = torch.autograd.grad(residual_block_norm(r, b, post), [post.weight], d)
+    (db,) = torch.autograd.grad(residual_block_norm(r, b, post), [post.bias], d)
+    all_ = torch.autograd.grad(residual_block_norm(r, b, post), [post.weight, post.bias], d)
+    assert torch.equal(dw, all_[0]) and torch.equal(db, all_[1])
+
+
+def test_forward_mode_is_refused():
+    x = torch.randn(4, 64, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(_lib.MtcError, match="forward-mode"):
+            block_norm(dual)
+        with pytest.raises(_lib.MtcError, match="forward-mode"):
+            residual_block_norm(x, x, gate=dual)

@@ -263,6 +263,20 @@ def test_refusals_on_the_gpu():
         global_norm([torch.eye(4, device=DEV).to_sparse()])
 
 
+def test_outputs_that_overlap_through_a_copy_are_refused():
+    """Outputs of another layout are written by a copy behind the kernel: also those must not share memory."""
+    t = [torch.randn(4, 6, device=DEV) for _ in range(2)]
+    buf = torch.zeros(4, 24, device=DEV)
+    with pytest.raises(_lib.MtcError, match="span the same memory"):
+        clip_by_global_norm_(t, 1.0, out=[buf[:, 0:12:2], buf[:, 2:14:2]])
+    with pytest.raises(_lib.MtcError, match="span the same memory"):
+        clip_by_global_norm_(t, 1.0, out=[buf[:, :6], buf.view(-1)[:24].view(4, 6)])
+    assert not bool(buf.any())
+    own = torch.zeros(8, 24, device=DEV)                             # rows with gaps, one block behind the other: apart
+    n = clip_by_global_norm_(t, 1e9, out=[own[:4, 2:8], own[4:, 2:8]])
+    assert torch.equal(own[:4, 2:8], t[0]) and torch.equal(own[4:, 2:8], t[1]) and float(n) > 0
+
+
 # ------------------------------------------------------------------------------------------------ in the optimizer
 def _cfg(dt, unit=True, **kw):
     return dict(dict(seed=49, prefix_sizes=[128, 384, 896, 2048], act_size=256, top_k=16, top_k_aux=64, aux_penalty=1 / 32,

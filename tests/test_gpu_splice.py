@@ -249,3 +249,24 @@ def test_store_harvests_through_the_norm():
     for _ in range(3):
         s, t = store.next_batch()
         assert torch.equal(s, want[t[:, 0].long()])
+
+
+@pytest.mark.parametrize("train", [True, False])
+def test_two_reconstructions_before_the_backward(train):
+    """Gradient accumulation and a block used twice: each call keeps its own selection."""
+    m = _transcoder(torch.float32, False).train(train)
+    if not train:
+        m.threshold.fill_(0.3)
+    xs = [torch.randn(n, 64, generator=torch.Generator("cpu").manual_seed(n)).to(DEV).requires_grad_(True) for n in (9, 30)]
+    ds = [torch.randn(n, 64, generator=torch.Generator("cpu").manual_seed(n + 1)).to(DEV) for n in (9, 30)]
+    leaves = [m.W_enc, m.b_enc, m.W_dec, m.b_dec]
+    outs = [m.reconstruct(x) for x in xs]
+    both = torch.autograd.grad(outs, xs + leaves, ds, retain_graph=True)
+    again = torch.autograd.grad(outs, xs + leaves, ds)                # the graph kept: the same bits
+    alone = [torch.autograd.grad(m.reconstruct(x), [x] + leaves, d) for x, d in zip(xs, ds)]
+    for a, b in zip(both, again):
+        assert torch.equal(a, b)
+    assert torch.equal(both[0], alone[0][0]) and torch.equal(both[1], alone[1][0])
+    for got, a, b in zip(both[2:], alone[0][1:], alone[1][1:]):
+        # one fp32 sum of the same two gradients, in either order
+        assert torch.equal(got, a + b)
