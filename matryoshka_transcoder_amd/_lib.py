@@ -172,6 +172,7 @@ def torch_binding():
     global _BINDING
     if _BINDING is None:
         lib = load()
+        import torch                                     # noqa: F401  the binding links against torch's libraries: they have to be loaded
         try:
             from . import _torch_binding
         except ImportError as e:

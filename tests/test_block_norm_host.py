@@ -1,6 +1,9 @@
 """What the block norms refuse before any launch (no GPU needed)."""
 import ctypes as C
 import json
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -96,3 +99,9 @@ def test_a_run_with_a_source_norm_can_be_saved(tmp_path):
     assert saved["source_norm"].startswith("BlockNorm(64, kind='rms'")
     with pytest.raises(_lib.MtcError, match="source_norm"):                 # what was saved is no module any more
         TranscoderActivationsStore(None, dict(cfg, source_norm=saved["source_norm"]))
+
+
+def test_the_binding_loads_in_a_process_without_torch():
+    """`_lib` itself imports no torch: the binding brings the libraries it links against."""
+    code = "from matryoshka_transcoder_amd import _lib; assert _lib.torch_binding() is _lib.torch_binding()"
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=str(Path(__file__).resolve().parents[1]))
