@@ -564,9 +564,11 @@ int mtc_comm_all_gather(mtc_comm* c, const void* send, void* recv, size_t send_c
  * normed is made from the fp32 sum, before hidden's rounding to the model dtype.  All operands in `dtype`; w / b of a norm
  * may be NULL (scale 1 instead of offset + w, bias 0).  gate: [A] (CHANNEL), one value per row at stride ld_gate (ROW),
  * [rows][A] (FULL) or one value (SCALAR).  ld_*: row strides in elements, columns are contiguous; 0 repeats one row (inputs).  Any width
- * 1 .. 8192, stride and alignment; 16-byte accesses when the width is a multiple of 8 and every row starts at a multiple of
- * 16 bytes, single elements otherwise.  Outputs must not overlap inputs.
- * stats (optional, float [rows][4], 16-byte aligned: post mean, post 1/std, pre mean, pre 1/std; zeros for absent norms) is what the backward needs.  rows = 0 is a no-op. */
+ * 1 .. 8192, stride and alignment; 16-byte accesses when a row is a multiple of 16 bytes long and every row starts at a
+ * multiple of 16 bytes, single elements otherwise.  Squares are summed in fp32: entries beyond about 1e19 (their square leaves
+ * its range) make a row's 1/std 0.  Outputs must not overlap inputs.
+ * stats (optional, float [rows][4], 16-byte aligned: post mean, post 1/std, pre mean, pre 1/std; zeros for absent norms) is
+ * what the backward needs.  rows = 0 is a no-op. */
 enum { MTC_NORM_NONE = 0, MTC_NORM_RMS = 1, MTC_NORM_LAYER = 2 };
 enum { MTC_GATE_NONE = 0, MTC_GATE_CHANNEL = 1, MTC_GATE_ROW = 2, MTC_GATE_FULL = 3, MTC_GATE_SCALAR = 4 };
 typedef struct mtc_block_norm_desc {

@@ -12,7 +12,7 @@
 // Layout: thread t of a row's T = 64 * ceil(A / 512) threads owns 8 columns for the whole launch, so the norm weights,
 // the channel gate and the column sums of the weight gradients live in its registers while it walks over rows.  A
 // workgroup holds `groups` such row groups.  Row sums: DPP inside a wave, one LDS exchange across the row's waves.
-// Rows whose width is a multiple of 8 with 16-byte-aligned rows use 16-byte accesses (columns 8 t .. 8 t + 7); any other
+// Rows of a multiple of 16 bytes that start at multiples of 16 bytes use 16-byte accesses (columns 8 t .. 8 t + 7); any other
 // width or stride takes the same kernel with single elements (columns t, t + T, ..., which keeps a wave's accesses side by side).
 #include <algorithm>
 #include <type_traits>
@@ -481,6 +481,10 @@ __global__ __launch_bounds__(256, (BRANCH && NU <= 5 ? 4 : 1)) void block_norm_w
 // and the column sums (over rows) X1 = gate D u_p, X2 = gate D, X3 = g u, X4 = g, from which block_norm_cols_kernel makes the
 // gradients of the weights, biases and the channel gate.  Each workgroup leaves one partial per column, summed in a
 // fixed order afterwards: no atomics, the same bits on every run.
+// One workgroup per CU of up to 768 threads (168 registers each, so that the column sums, the weights and two rows' operands fit),
+// several row groups in it where rows are short; its groups' sums meet in LDS.  Bound by memory at large sizes: 16384 x 4608 bf16
+// pair with a channel gate 163 us with the column kernel (5.6 TB/s over its six operands), 16384 x 2304 83 us (5.5); by the
+// operands' latency at small ones: 1024 x 2304 15 us.  A third row's operands in flight spill: 16384 x 1600 fp32 115 -> 167 us.
 template <typename COLS, bool FULL> struct BwdRow {
     typename COLS::Raw branch, gate[FULL ? 1 : 0], d_hidden, residual, d_normed;
     uint32_t gr;
@@ -675,7 +679,8 @@ struct NormCols {
     int want_x1, want_x2, want_scalar;
 };
 
-// the last sums over the workgroups' partials: 64 columns per workgroup, its 16 waves share the partials
+// the last sums over the workgroups' partials: 64 columns per workgroup, its 16 waves share the partials.  Bound by latency
+// (width 4608: 13 MB of partials in 5 us)
 template <int DT>
 __global__ __launch_bounds__(1024) void block_norm_cols_kernel(NormCols n) {
     typedef typename DType<DT>::T T_;

@@ -60,7 +60,8 @@ def clip_by_global_norm_(tensors: Tensors, max_norm: float, norm_type: float = 2
     """Scale the tensors in place so that their common norm is at most max_norm; returns the norm before (float32 scalar).
 
     out: tensors of the same shapes and dtypes that receive the scaled values instead; the inputs then stay as they are.
-    Dense tensors (and outputs) that share memory with one another are refused.  Nothing is written, in place, when the norm
+    Dense tensors (and outputs) that share memory with one another are refused; outputs laid out unlike their inputs are written by
+    a copy, and must not span the same memory as any other output.  Nothing is written, in place, when the norm
     is within the limit.  error_if_nonfinite: raise before anything is changed if the norm is not finite (reads it back: a
     synchronisation)."""
     src = _list(tensors)
