@@ -66,7 +66,8 @@ class TranscoderActivationsStore:
     def __init__(self, model, cfg: dict, source=None, token_iterator: Optional[Iterator] = None):
         """cfg["source_norm"] (optional, a block_norm.BlockNorm on the GPU): the harvested source is the residual stream in
         front of a block, and the block's own norm of it becomes the transcoder's source activation -- one stream to
-        harvest or store instead of two, for models that have no hook behind that norm."""
+        harvest or store instead of two, for models that have no hook behind that norm.  cfg["source_hook_point"] then has to
+        be a point in front of the norm, and the model has to expose it: what a norm has left already is refused."""
         self.model = model
         self.source_norm = cfg.get("source_norm")
         if self.source_norm is not None and not isinstance(self.source_norm, torch.nn.Module):
@@ -74,6 +75,9 @@ class TranscoderActivationsStore:
         self.config = cfg
         self.device = cfg["device"]
         self.source_hook_point = cfg.get("source_hook_point")
+        if self.source_norm is not None and str(self.source_hook_point).endswith("hook_normalized"):
+            raise _lib.MtcError(f"cfg['source_norm'] norms the residual stream, but {self.source_hook_point} (hook_normalized) lies "
+                                "behind a norm")
         self.target_hook_point = cfg.get("target_hook_point")
         self.model_batch_size = cfg.get("model_batch_size", 512)
         self.num_batches_in_buffer = cfg.get("num_batches_in_buffer", 10)
@@ -102,7 +106,8 @@ class TranscoderActivationsStore:
     def get_paired_activations(self, batch_tokens: torch.Tensor):
         names = [self.target_hook_point, self.source_hook_point]
         fallback, layer = None, None
-        if self.source_hook_point and "hook_mlp_in" in self.source_hook_point:
+        # the fallback is what the block's own norm left: nothing that cfg["source_norm"] may be applied to
+        if self.source_hook_point and "hook_mlp_in" in self.source_hook_point and self.source_norm is None:
             layer = int(self.source_hook_point.split(".")[1])
             fallback = f"blocks.{layer}.ln2.hook_normalized"
             names.append(fallback)
@@ -112,7 +117,10 @@ class TranscoderActivationsStore:
             src = cache[self.source_hook_point]
         except KeyError:
             if fallback is None:
-                raise
+                if self.source_norm is None:
+                    raise
+                raise _lib.MtcError(f"the model does not expose {self.source_hook_point}: with cfg['source_norm'], name a hook of the "
+                                    "residual stream that it has as source_hook_point") from None
             ln2 = self.model.blocks[layer].ln2
             scale = next((getattr(ln2, a) for a in ("w", "weight", "scale", "g") if hasattr(ln2, a)), None)
             src = cache[fallback] if scale is None else cache[fallback] * scale
