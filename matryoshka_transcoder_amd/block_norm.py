@@ -57,6 +57,21 @@ class BlockNorm(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return _call(x, None, None, None, self, 1.0, 1.0)[1]
 
+    def saved_form(self) -> dict:
+        """Everything the norm consists of, for a file (numbers, text and tensors only); `from_saved` makes it again."""
+        return {"spec": {"width": self.width, "kind": self.kind, "eps": self.eps, "weight_offset": self.weight_offset,
+                         "affine": self.weight is not None, "bias": self.bias is not None},
+                "state_dict": {k: v.detach().clone() for k, v in self.state_dict().items()}}
+
+    @classmethod
+    def from_saved(cls, saved: dict, device=None) -> "BlockNorm":
+        if "spec" not in saved:
+            raise MtcError("the saved source_norm is not a BlockNorm and cannot be made again from its file")
+        state, spec = saved["state_dict"], dict(saved["spec"])
+        norm = cls(spec.pop("width"), **spec, dtype=state["weight"].dtype if "weight" in state else None, device=device)
+        norm.load_state_dict(state)
+        return norm
+
     def extra_repr(self) -> str:
         return (f"{self.width}, kind={self.kind!r}, eps={self.eps}, weight_offset={self.weight_offset}, "
                 f"affine={self.weight is not None}, bias={self.bias is not None}")

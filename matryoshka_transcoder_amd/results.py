@@ -8,7 +8,9 @@
 What the reference does not persist goes to a side file `checkpoints/{name}.extra.pt`, so that the reference layout
 stays loadable by the reference: always `step` and the dead counters (`num_batches_not_active`), plus the optimizer's
 `state_dict()` (Adam moments and step counts) when `save_checkpoint` is given the optimizer -- `train_transcoder`
-passes it.  `load_extra` restores all of it (tensors only, `weights_only=True`): a resumed run continues bit for bit.
+passes it.  `load_checkpoint` restores all of it (tensors only, `weights_only=True`): a resumed run continues bit for bit.
+A run with cfg["source_norm"] also leaves that norm, weights included, in `checkpoints/{name}.source_norm.pt`: config.json can
+only describe it, and whoever uses the run (sae_bench.build_matryoshka_adapter) has to apply it.
 """
 from __future__ import annotations
 
@@ -18,6 +20,13 @@ from pathlib import Path
 from typing import Any, Dict, Optional
 
 import torch
+
+from .block_norm import BlockNorm
+
+
+def source_norm_path(weights: Path) -> Path:
+    """Where the source norm of a run lies whose weights are in `weights` (no file: the run had none)."""
+    return weights.with_name(f"{weights.stem}.source_norm.pt")
 
 
 def _jsonable(obj: Any) -> Any:
@@ -64,6 +73,11 @@ class CleanResultsManager:
             extra["optimizer"] = optimizer.state_dict()
         if extra:
             torch.save(extra, weights.with_name(f"{stem}.extra.pt"))
+        norm = config.get("source_norm")
+        if isinstance(norm, torch.nn.Module):
+            torch.save(norm.saved_form() if isinstance(norm, BlockNorm) else {"state_dict": norm.state_dict()}, source_norm_path(weights))
+        elif norm is None:
+            source_norm_path(weights).unlink(missing_ok=True)        # an earlier run's in the same place
         cfg_out = dict(config)
         cfg_out.pop("completed_at", None)
         if is_final:

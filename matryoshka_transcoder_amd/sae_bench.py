@@ -20,7 +20,10 @@ from typing import Any, Iterable, Mapping, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from ._lib import MtcError
+from .block_norm import BlockNorm
 from .config import compute_fvu, get_hook_name
+from .results import source_norm_path
 from .transcoder import MatryoshkaTranscoder
 
 
@@ -132,7 +135,10 @@ def _valid_top_k(top_k: int, dict_size: int) -> int:
 
 # ------------------------------------------------------------------ adapters
 class MatryoshkaAutoInterpAdapter(MatryoshkaTranscoder):
-    """`MatryoshkaTranscoder` + the attributes SAEBench expects on an SAE (wrappers.py:53-109)."""
+    """`MatryoshkaTranscoder` + the attributes SAEBench expects on an SAE (wrappers.py:53-109).
+
+    A run trained with cfg["source_norm"] saw the norm of what its hook yields: the adapter keeps a frozen copy of that norm
+    (`source_norm`, not among its parameters: the state_dict stays the reference's) and applies it to every source it is given."""
 
     def __init__(self, cfg: dict, *, sae_cfg: AutoInterpSAEConfig) -> None:
         own = copy.deepcopy(dict(cfg))
@@ -141,6 +147,14 @@ class MatryoshkaAutoInterpAdapter(MatryoshkaTranscoder):
         own["top_k"] = _valid_top_k(int(own.get("top_k", width)), width)
         own["top_k_aux"] = max(own["top_k"], int(own.get("top_k_aux", 2 * own["top_k"])))
         own.setdefault("n_batches_to_dead", 20)
+        norm = own.get("source_norm")
+        if norm is not None and not isinstance(norm, torch.nn.Module):
+            raise MtcError(f"cfg['source_norm'] must be the run's norm as a module, got {norm!r}")
+        if norm is not None and str(sae_cfg.hook_name).endswith("hook_normalized"):
+            raise MtcError(f"the run norms its source itself (cfg['source_norm']), but {sae_cfg.hook_name} (hook_normalized) lies behind a norm")
+        if isinstance(norm, BlockNorm) and norm.width != sae_cfg.d_in:
+            raise MtcError(f"source_norm of width {norm.width} in front of a transcoder of width {sae_cfg.d_in}")
+        self._source_norm = (None if norm is None else norm.requires_grad_(False),)        # own is a copy
         super().__init__(own)
         self.cfg = sae_cfg
         self.device = torch.device(own["device"])
@@ -154,6 +168,30 @@ class MatryoshkaAutoInterpAdapter(MatryoshkaTranscoder):
         if "device" in kwargs:
             self.device = torch.device(kwargs["device"])
         return moved
+
+    @property
+    def source_norm(self):
+        return self._source_norm[0]
+
+    def _apply(self, fn, *args, **kwargs):
+        if self.source_norm is not None:
+            self.source_norm._apply(fn, *args, **kwargs)
+        return super()._apply(fn, *args, **kwargs)
+
+    def _normed(self, x_source):
+        return x_source if self.source_norm is None else self.source_norm(x_source)
+
+    def encode(self, x_source):
+        return super().encode(self._normed(x_source))
+
+    def reconstruct(self, x_source):
+        return super().reconstruct(self._normed(x_source))
+
+    def compute_activations(self, x_source):
+        return super().compute_activations(self._normed(x_source))
+
+    def _run_forward(self, x_source, *args):
+        return super()._run_forward(self._normed(x_source), *args)
 
     def get_decoder_row_norms(self) -> torch.Tensor:
         return self.W_dec.detach().norm(dim=-1)
@@ -175,8 +213,17 @@ class MatryoshkaAutoInterpAdapter(MatryoshkaTranscoder):
 def build_matryoshka_adapter(cfg: Mapping[str, Any], *, state_dict_path=None, hook_layer: Optional[int] = None,
                              hook_point: Optional[str] = None) -> MatryoshkaAutoInterpAdapter:
     """wrappers.py:118-156: adapter from a training config (+ optionally a saved state_dict); decoder rows are
-    re-normalised after loading."""
+    re-normalised after loading.  The run's source norm is cfg["source_norm"] where that is the module; a saved run brings its
+    own (results.py), for a configuration read back from config.json or one that does not name it.  None: the adapter norms
+    nothing (its hook yields normed activations)."""
     own = copy.deepcopy(dict(cfg))
+    if "source_norm" not in own or isinstance(own["source_norm"], str):
+        saved = None if state_dict_path is None else source_norm_path(Path(state_dict_path))
+        if saved is not None and saved.exists():
+            own["source_norm"] = BlockNorm.from_saved(torch.load(saved, map_location="cpu", weights_only=True))
+        elif "source_norm" in own:
+            raise MtcError(f"the run's source_norm ({own['source_norm']}) is only described: pass it as a module, or the checkpoint it was "
+                           "saved beside")
     layer = own.get("source_layer", own["layer"]) if hook_layer is None else hook_layer
     point = hook_point or own.get("source_hook_point") or get_hook_name(own["source_site"], layer, own["model_name"])
     sae_cfg = AutoInterpSAEConfig.from_kwargs(
