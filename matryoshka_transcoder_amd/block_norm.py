@@ -100,7 +100,8 @@ def residual_block_norm(residual: torch.Tensor, branch: torch.Tensor, post: Opti
     residual and branch: one shape [..., width], one dtype (float32 or bfloat16), one GPU; leading dimensions may be strided
     or expanded.  gate: a scalar tensor, [width] (per channel), [..., 1] (per token) or the full shape.
     Differentiable in residual, branch, gate and both norms' parameters, once: a backward with create_graph = True raises, and
-    so do forward-mode tangents and a backward recorded into a HIP graph while an eager graph of the same leaves is alive."""
+    so do forward-mode tangents, tracing (torch.jit.trace, make_fx) and a backward recorded into a HIP graph while an eager graph of
+    the same leaves is alive."""
     hidden, normed = _call(residual, branch, gate, post, pre, residual_scale, branch_scale)
     return hidden if pre is None else (hidden, normed)
 

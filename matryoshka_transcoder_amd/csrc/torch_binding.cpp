@@ -4,7 +4,10 @@
 // engine's thread, 150 us forward and backward.  No kernel is here: everything computes in libmtc.so, whose entry
 // points are handed over by address (bind), so that this module and ctypes drive the one library that is loaded.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -50,6 +53,14 @@ struct Lib {
 
 void check(int rc, const char* what) {
     if (rc) fail(what, " failed (", rc, "): ", lib.last_error());
+}
+
+// What records torch operations (jit.trace, make_fx, export and what builds on them) sees an output's allocation and nothing of the kernel
+// that fills it: the record would return memory that nobody wrote.
+void refuse_tracing(const char* what) {
+    if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+        fail(what, " cannot be traced (torch.jit.trace, make_fx): the kernel would be missing from the trace");
 }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
@@ -216,6 +227,7 @@ std::tuple<OptTensor, OptTensor> block_norm(const Tensor& residual, const OptTen
                                             const OptTensor& post_w, const OptTensor& post_b, double post_eps, double post_off,
                                             int64_t post_width, int pre_kind, const OptTensor& pre_w, const OptTensor& pre_b, double pre_eps,
                                             double pre_off, int64_t pre_width, double rs, double bs) {
+    refuse_tracing("a block norm");
     if (!residual.is_cuda())
         fail("the block norms run on the GPU only (HIP kernels); got a ", residual.device(), " tensor and there is no CPU fallback");
     if (residual.dim() < 1) fail("a norm needs a tensor with at least one dimension");
@@ -303,6 +315,7 @@ std::vector<Tensor> dense(const std::vector<Tensor>& ts) {
 
 // {norm, coef} (fp32), or with `raw` the sum before the root (fp64)
 Tensor norm_of(const std::vector<Tensor>& ts, double order, double max_norm, bool raw) {
+    refuse_tracing("a gradient norm");
     const float p = norm_order(order), limit = norm_limit(max_norm);
     check_gradients(ts);
     if (ts.empty()) fail("no gradients to take a norm of");
@@ -339,6 +352,7 @@ void check_copied_outputs(const std::vector<Tensor>& dst, const std::vector<Tens
 }
 
 Tensor clip(const std::vector<Tensor>& src, const std::optional<std::vector<Tensor>>& out, double order, double max_norm) {
+    refuse_tracing("gradient clipping");
     const float p = norm_order(order), limit = norm_limit(max_norm);
     const std::vector<Tensor>& dst = out.has_value() ? *out : src;
     check_gradients(src);
@@ -406,5 +420,6 @@ PYBIND11_MODULE(_torch_binding, m) {
     });
     m.def("block_norm", &block_norm, py::call_guard<py::gil_scoped_release>());
     m.def("norm_of", &norm_of, py::call_guard<py::gil_scoped_release>());
+    m.def("refuse_tracing", &refuse_tracing);
     m.def("clip", &clip, py::call_guard<py::gil_scoped_release>());
 }

@@ -40,6 +40,7 @@ def power_sum(tensors: Tensors, norm_type: float = 2.0) -> torch.Tensor:
 
 def coef_of_power_sum(total: torch.Tensor, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """`norm_and_coef` of gradients whose combined `power_sum` is `total`."""
+    _lib.torch_binding().refuse_tracing("a gradient norm")
     if not total.is_cuda or total.dtype != torch.float64 or total.numel() != 1:
         raise MtcError("total must be one float64 value on the GPU")
     with torch.cuda.device(total.device):

@@ -539,6 +539,7 @@ class MatryoshkaTranscoder(nn.Module):
         parameters: what a model's block needs when the transcoder stands in for its MLP (splice.py).  Any leading shape;
         honours train / eval mode as `encode` does (in train mode the global TopK moves the threshold's average; the dead
         counters stay).  Statistics of the input standardisation are kept like `encode`'s and take part in the gradient."""
+        _lib.torch_binding().refuse_tracing("reconstruct()")
         self._check_inputs(x_source)
         if x_source.shape[-1] != self.source_act_size:
             raise _lib.MtcError(f"reconstruct() needs activations of width {self.source_act_size}, got {list(x_source.shape)}")
