@@ -62,6 +62,14 @@ class _StepFn(torch.autograd.Function):
         return None, None, None, dW_encT.t(), db_enc, dW_dec, db_dec
 
 
+def _refuse_recording():
+    """The select keeps its bound from call to call (training) or reads a size back (eval), the feature-major index is cleared by a
+    memset, which a replay need not repeat before the counts are added up, and a live eager graph of the parameters, made on
+    the default stream, ends a process that records their backward: nothing of this belongs into a HIP graph."""
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.MtcError("reconstruct() cannot be recorded into a HIP graph, neither forward nor backward: record what stands around it")
+
+
 class _ReconstructFn(torch.autograd.Function):
     """Standardised input -> selected features -> reconstruction, for any incoming gradient (the training step's own backward,
     _StepFn, starts from its loss).  Gradients flow through the selected features only, as in sae.py:173-191."""
@@ -83,6 +91,7 @@ class _ReconstructFn(torch.autograd.Function):
         x, W_enc, W_dec = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[1], any(ctx.needs_input_grad[2:6])
         with module._on_device():
+            _refuse_recording()
             hp = module.hot_path()
             d = hp.desc(x.shape[0])
             g = g.contiguous()
@@ -538,7 +547,8 @@ class MatryoshkaTranscoder(nn.Module):
         """`decode(encode(x_source))` (sae.py:363-406) without the dense feature tensor, differentiable in x_source and the
         parameters: what a model's block needs when the transcoder stands in for its MLP (splice.py).  Any leading shape;
         honours train / eval mode as `encode` does (in train mode the global TopK moves the threshold's average; the dead
-        counters stay).  Statistics of the input standardisation are kept like `encode`'s and take part in the gradient."""
+        counters stay).  Statistics of the input standardisation are kept like `encode`'s and take part in the gradient.  Not inside
+        a trace or a HIP graph (refused)."""
         _lib.torch_binding().refuse_tracing("reconstruct()")
         self._check_inputs(x_source)
         if x_source.shape[-1] != self.source_act_size:
@@ -552,6 +562,7 @@ class MatryoshkaTranscoder(nn.Module):
         params = (self.W_enc, self.b_enc, self.W_dec, self.b_dec)
         unit = bool(self.config.get("input_unit_norm", False))
         with self._on_device():
+            _refuse_recording()
             if not unit:
                 self.x_mean = self.x_std = None
                 return _ReconstructFn.apply(self, x, *params, None, None).reshape(lead + (-1,))

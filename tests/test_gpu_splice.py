@@ -270,3 +270,29 @@ def test_two_reconstructions_before_the_backward(train):
     for got, a, b in zip(both[2:], alone[0][1:], alone[1][1:]):
         # one fp32 sum of the same two gradients, in either order
         assert torch.equal(got, a + b)
+
+
+@pytest.mark.parametrize("train", [True, False])
+def test_recording_into_a_graph_is_refused(train):
+    """Forward and backward, before anything is launched; afterwards the same calls work as before."""
+    m = _transcoder(torch.float32, True).train(train)
+    x = torch.randn(5, 64, generator=torch.Generator("cpu").manual_seed(8)).to(DEV).requires_grad_(True)
+    b = SplicedTranscoder(m, BlockNorm(64, device=DEV))
+    with torch.no_grad():
+        want = m.reconstruct(x).clone()
+    for call in (m.reconstruct, b):
+        with pytest.raises(_lib.MtcError, match="recorded into a HIP graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()), torch.no_grad():
+                call(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = m.reconstruct(x)
+        g = torch.ones_like(out)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.MtcError, match="recorded into a HIP graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            torch.autograd.grad(out, [x], g)
+    with torch.no_grad():
+        assert torch.equal(m.reconstruct(x), want)
