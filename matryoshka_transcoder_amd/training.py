@@ -69,6 +69,12 @@ class FusedAdam(torch.optim.Optimizer):
         self.last_grad_norm = None
         super().__init__(list(transcoder.parameters()), dict(lr=lr, betas=betas, eps=eps))
 
+    @staticmethod
+    def _moved(*tensors):
+        """The kernels write parameters behind autograd's back: a graph that saved one of them (MatryoshkaTranscoder.reconstruct) has
+        to notice, as after any in-place operation, instead of using the new values in its backward."""
+        torch.autograd.graph.increment_version(tensors)
+
     def _state(self, p):
         st = self.state[p]
         if not st:
@@ -154,6 +160,7 @@ class FusedAdam(torch.optim.Optimizer):
             torch.cuda.current_stream().wait_event(e_b)     # every later reader of b_dec / g / the scalars is ordered behind the side stream
         else:
             update_b_dec()
+        self._moved(tc.W_dec, tc.W_enc, tc.b_enc, tc.b_dec)
         return tc._output_dict(res, x_target)               # (flushes what the forward chain deferred behind the backward launches)
 
     def _dense_step(self, res, x_target):
@@ -209,6 +216,7 @@ class FusedAdam(torch.optim.Optimizer):
                 else:
                     g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
                     hp.adam_flat(p.data, g, st["exp_avg"], st["exp_avg_sq"], h, grad_scale=scale)
+                self._moved(p)
         return None
 
 

@@ -244,6 +244,7 @@ class MatryoshkaTranscoder(nn.Module):
             self.W_dec.grad = self.W_dec.grad.contiguous()
         with self._on_device():
             self.hot_path().unitnorm_project(self.W_dec.data, self.W_dec.grad)
+        torch.autograd.graph.increment_version((self.W_dec, self.W_dec.grad))       # written by a kernel: graphs that saved them notice
 
     @torch.no_grad()
     def update_inactive_features(self, acts):

@@ -296,3 +296,24 @@ def test_recording_into_a_graph_is_refused(train):
             torch.autograd.grad(out, [x], g)
     with torch.no_grad():
         assert torch.equal(m.reconstruct(x), want)
+
+
+@pytest.mark.parametrize("how", ["step", "step_project", "train_step", "unit_norm"])
+def test_a_backward_after_the_parameters_moved_is_refused(how):
+    """A graph made before an update must not take the new weights for the old ones (torch's own in-place check)."""
+    m = _transcoder(torch.float32, False).train()
+    opt = FusedAdam(m, lr=1e-3)
+    x = torch.randn(16, 64, generator=torch.Generator("cpu").manual_seed(9)).to(DEV)
+    m.reconstruct(x).sum().backward()                                    # gradients for the update
+    out = m.reconstruct(x)
+    if how == "unit_norm":
+        m.make_decoder_weights_and_grad_unit_norm()
+    elif how == "train_step":
+        opt.train_step(x, x)
+    else:
+        opt.step(project=how == "step_project")
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    opt.zero_grad()
+    m.reconstruct(x).sum().backward()                                    # the next forward and backward are as ever
+    assert m.W_dec.grad is not None
