@@ -102,6 +102,8 @@ def residual_block_norm(residual: torch.Tensor, branch: torch.Tensor, post: Opti
     Differentiable in residual, branch, gate and both norms' parameters, once: a backward with create_graph = True raises, and
     so do forward-mode tangents, tracing (torch.jit.trace, make_fx) and a backward recorded into a HIP graph while an eager graph of
     the same leaves is alive."""
+    if branch is None:
+        raise MtcError("residual_block_norm needs a branch: block_norm (or a BlockNorm) norms the residual alone")
     hidden, normed = _call(residual, branch, gate, post, pre, residual_scale, branch_scale)
     return hidden if pre is None else (hidden, normed)
 

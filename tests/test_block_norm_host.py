@@ -105,3 +105,11 @@ def test_the_binding_loads_in_a_process_without_torch():
     """`_lib` itself imports no torch: the binding brings the libraries it links against."""
     code = "from matryoshka_transcoder_amd import _lib; assert _lib.torch_binding() is _lib.torch_binding()"
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=str(Path(__file__).resolve().parents[1]))
+
+
+def test_a_residual_without_a_branch_is_refused():
+    """residual_block_norm adds a branch; a norm of the residual alone is block_norm's (and hidden would be nothing)."""
+    x = torch.randn(4, 64)
+    for kw in ({}, dict(pre=BlockNorm(64)), dict(post=BlockNorm(64)), dict(gate=torch.ones(()))):
+        with pytest.raises(_lib.MtcError, match="branch"):
+            residual_block_norm(x, None, **kw)
