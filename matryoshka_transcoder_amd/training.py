@@ -186,7 +186,7 @@ class FusedAdam(torch.optim.Optimizer):
     def _step(self, project: bool):
         tc = self.transcoder
         hp = tc.hot_path()
-        scale = None
+        scale = self.last_grad_norm = None
         if self.max_grad_norm is not None:
             live = [p for group in self.param_groups for p in group["params"] if p.grad is not None]
             if live:

@@ -430,3 +430,20 @@ def test_sharded_norm_is_the_whole_dictionary_s(world):
         assert _close(ret["norms0"][i], float(o.last_grad_norm), 1e-4) and float(o.last_grad_norm) > 0.01
     for k, v in ret["sd"].items():
         assert float((v - m.state_dict()[k].cpu()).abs().max()) <= 1e-2 * 3e-4 * 3, k       # the fp32 bar of the sharded step
+
+
+def test_a_step_without_gradients_leaves_no_old_norm():
+    """last_grad_norm is the last step's: nothing was clipped in a step that found no gradients."""
+    from matryoshka_transcoder_amd.training import FusedAdam
+    from matryoshka_transcoder_amd.transcoder import MatryoshkaTranscoder
+    cfg = dict(seed=49, prefix_sizes=[32, 128], act_size=64, top_k=8, top_k_aux=32, aux_penalty=1 / 32, n_batches_to_dead=20, l1_coeff=0.0,
+               dtype=torch.float32, device=DEV, input_unit_norm=False, lr=3e-4, beta1=0.9, beta2=0.99)
+    tc = MatryoshkaTranscoder(cfg)
+    opt = FusedAdam(tc, lr=1e-3, max_grad_norm=0.5)
+    for p in tc.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert float(opt.last_grad_norm) > 0
+    opt.zero_grad()
+    opt.step()
+    assert opt.last_grad_norm is None
