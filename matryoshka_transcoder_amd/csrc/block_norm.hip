@@ -365,17 +365,28 @@ template <int DT, int NU> struct WaveRow {
         }
     }
 };
+// a lane's units added as a tree: with the 4 or 8 values of a unit one after another and 6 levels in the wave, a row sum has at
+// most 18 roundings in sequence for any NU, where one chain over the lane's columns would have up to 78
+template <int NU> __device__ __forceinline__ float units_total(float (&p)[NU]) {
+#pragma unroll
+    for (int s = 1; s < NU; s *= 2)
+#pragma unroll
+        for (int u = 0; u + s < NU; u += 2 * s) p[u] += p[u + s];
+    return wave_total(p[0]);
+}
 // v becomes v - mean (layer); returns 1/std
 template <int NU, int E>
 __device__ __forceinline__ float wave_normalise(float (&v)[NU][E], int kind, float eps, float inv_A, int lane, int A, float& mu) {
+    float p[NU];
     mu = 0.f;
     if (kind == MTC_NORM_LAYER) {
-        float s = 0.f;
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+        for (int u = 0; u < NU; ++u) {
+            p[u] = v[u][0];
 #pragma unroll
-            for (int i = 0; i < E; ++i) s += v[u][i];
-        mu = wave_total(s) * inv_A;
+            for (int i = 1; i < E; ++i) p[u] += v[u][i];
+        }
+        mu = units_total<NU>(p) * inv_A;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const float m = (u * 64 + lane) * E < A ? mu : 0.f;
@@ -383,12 +394,13 @@ __device__ __forceinline__ float wave_normalise(float (&v)[NU][E], int kind, flo
             for (int i = 0; i < E; ++i) v[u][i] -= m;
         }
     }
-    float q = 0.f;
 #pragma unroll
-    for (int u = 0; u < NU; ++u)
+    for (int u = 0; u < NU; ++u) {
+        p[u] = v[u][0] * v[u][0];
 #pragma unroll
-        for (int i = 0; i < E; ++i) q = fmaf(v[u][i], v[u][i], q);
-    return 1.f / sqrtf(fmaf(wave_total(q), inv_A, eps));
+        for (int i = 1; i < E; ++i) p[u] = fmaf(v[u][i], v[u][i], p[u]);
+    }
+    return 1.f / sqrtf(fmaf(units_total<NU>(p), inv_A, eps));
 }
 
 template <int DT, int NU, bool BRANCH, bool PRE, bool PLAIN>

@@ -477,3 +477,29 @@ def test_forward_mode_is_refused():
             block_norm(dual)
         with pytest.raises(_lib.MtcError, match="forward-mode"):
             residual_block_norm(x, x, gate=dual)
+
+
+@pytest.mark.parametrize("dt,A,branch", [(torch.bfloat16, 4608, False), (torch.bfloat16, 2304, True), (torch.float32, 2304, False),
+                                         (torch.float32, 1280, True), (torch.bfloat16, 4608, True), (torch.bfloat16, 1001, True)])
+def test_row_sums_lose_what_their_tree_loses(dt, A, branch):
+    """One entry that swallows whatever is added to it alone: a row's sum may lose at most 18 half steps (8 adds in a run of columns,
+    4 levels over a thread's runs or the row's waves, 6 in a wave), however many columns a thread holds.  The mean is that and
+    1 / A and its product: 20.  1/std: half of 18 (the root), 1 / A and the sum with eps (half each), the root, the quotient: 12."""
+    from matryoshka_transcoder_amd.engine import _p, _stream
+    lib, u = _lib.load(), 2.0 ** -24 * 1.01
+    code = _lib.MTC_BF16 if dt == torch.bfloat16 else _lib.MTC_F32
+    for kind, small, which, bound in ((_lib.MTC_NORM_RMS, 2.0 ** -12, 1, 12), (_lib.MTC_NORM_LAYER, 2.0 ** -24, 0, 20)):
+        x = torch.full((3, A), small, dtype=dt, device=DEV)
+        for r, c in enumerate((0, 8, A - 1)):
+            x[r, c] = 1.0
+        x64 = x.double()
+        exact = x64.mean(1) if which == 0 else 1.0 / torch.sqrt((x64 * x64).mean(1) + float(torch.tensor(1e-6, dtype=torch.float32)))
+        out, zero = torch.empty_like(x), torch.zeros_like(x)
+        stats = torch.empty(3, 4, dtype=torch.float32, device=DEV)
+        d = _lib.BlockNormDesc(rows=3, A=A, dtype=code, has_branch=int(branch), residual_scale=1.0, branch_scale=1.0, post_eps=1e-6,
+                               pre_eps=1e-6, post_kind=kind if branch else 0, pre_kind=0 if branch else kind, ld_residual=A, ld_branch=A,
+                               ld_hidden=A, ld_normed=A)
+        _lib.check(lib.mtc_block_norm_fwd(C.byref(d), _p(zero if branch else x), _p(x) if branch else None, None, None, None, None, None,
+                                          _p(out) if branch else None, None if branch else _p(out), _p(stats), _stream()))
+        got = stats[:, which if branch else 2 + which].double()
+        assert bool(((got - exact).abs() <= bound * u * exact).all()), (kind, ((got - exact).abs() / (exact * 2.0 ** -24)).tolist())
