@@ -540,9 +540,10 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(NormArgs a) {
     for (int i = 0; i < 8; ++i) x1[i] = x2[i] = x3[i] = x4[i] = 0.f;
     walk_rows<PREFETCH>(base0, step, a.rows, fetch, first, [&](long long base, const Row& q) {
         // Groups behind the last row read zeros everywhere, 1/std among them: they add zeros and store nothing.
-        // The statistics are folded into the factors of fused multiply-adds, and work that only a layer norm, a row gate, a
+        // An RMS norm's 1/std is folded into the factors of fused multiply-adds, and work that only a layer norm, a row gate, a
         // gate's gradient or a residual scale needs sits behind branches that the whole launch takes alike: the loop is
-        // bound by the number of vector instructions once the loads are in flight in time.
+        // bound by the number of vector instructions once the loads are in flight in time.  A layer norm subtracts its mean
+        // first, from the sum as the forward made it: x rstd - mu rstd would round at the size of mu for rows far from zero.
         const bool live = base + group < a.rows;
         const long long row = live ? base + group : 0;
         const float rstd_p = a.post_kind == MTC_NORM_NONE ? 1.f : __uint_as_float(q.st[1]);
@@ -551,9 +552,9 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(NormArgs a) {
         if (BRANCH) {
             q.branch.unpack(up);
             if (a.post_kind == MTC_NORM_LAYER) {
-                const float k = -__uint_as_float(q.st[0]) * rstd_p;
+                const float mu = __uint_as_float(q.st[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) up[i] = fmaf(up[i], rstd_p, k);
+                for (int i = 0; i < 8; ++i) up[i] = (up[i] - mu) * rstd_p;
             } else if (a.post_kind == MTC_NORM_RMS) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) up[i] *= rstd_p;
@@ -564,15 +565,24 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(NormArgs a) {
             q.d_hidden.unpack(D);
         }
         if (PRE) {
-            const float rstd = __uint_as_float(q.st[3]), k = -__uint_as_float(q.st[2]) * rstd;
-            const float kr = BRANCH ? a.res_scale * rstd : rstd, kz = gr * rstd;
+            const float rstd = __uint_as_float(q.st[3]);
             float u[8], dn[8], s[2] = {0.f, 0.f};
             q.residual.unpack(u);
             q.d_normed.unpack(dn);
+            if (a.pre_kind == MTC_NORM_LAYER) {
+                const float mu = __uint_as_float(q.st[2]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (BRANCH) u[i] = fmaf(FULL ? g[i] : gr, z[i], a.res_scale * u[i]);
+                    u[i] = (u[i] - mu) * rstd;
+                }
+            } else {
+                const float kr = BRANCH ? a.res_scale * rstd : rstd, kz = gr * rstd;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] = BRANCH ? fmaf(kr, u[i], (FULL ? g[i] * rstd : kz) * z[i]) : kr * u[i];
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float zi = BRANCH ? fmaf(FULL ? g[i] * rstd : kz, z[i], k) : k;
-                u[i] = fmaf(kr, u[i], zi);
                 if (SUMS >= 1) x3[i] = fmaf(dn[i], u[i], x3[i]);
                 if (SUMS >= 2) x4[i] += dn[i];
                 dn[i] *= w.qw[i];

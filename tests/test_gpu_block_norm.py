@@ -503,3 +503,35 @@ def test_row_sums_lose_what_their_tree_loses(dt, A, branch):
                                           _p(out) if branch else None, None if branch else _p(out), _p(stats), _stream()))
         got = stats[:, which if branch else 2 + which].double()
         assert bool(((got - exact).abs() <= bound * u * exact).all()), (kind, ((got - exact).abs() / (exact * 2.0 ** -24)).tolist())
+
+
+@pytest.mark.parametrize("A", [776, 777, 7000])
+@pytest.mark.parametrize("mode", ["pre", "pair", "post"])
+def test_backward_of_layer_norms_far_from_zero(mode, A):
+    """The normalised entries that a layer norm's gradients are made of, rebuilt from the row, its mean and its 1/std: the difference is
+    exact for entries near the mean, so only the product rounds (and the difference, further away): two half steps of each entry,
+    wherever the row lies.  One row and an incoming gradient of ones: the weight's gradient is these entries."""
+    from matryoshka_transcoder_amd.engine import _p, _stream
+    lib = _lib.load()
+    g = torch.Generator("cpu").manual_seed(21)
+    x, y = (_rand(g, 1, A) + 4000.0).to(DEV), _rand(g, 1, A).to(DEV)
+    one, w, b = torch.ones(1, A, device=DEV), torch.ones(A, device=DEV), torch.zeros(A, device=DEV)
+    branch = {"pre": None, "pair": y, "post": x}[mode]
+    res = y if mode == "post" else x
+    hidden, normed, stats, dw = torch.empty_like(x), torch.empty_like(x), torch.empty(1, 4, device=DEV), torch.empty_like(w)
+    layer, pre, post = _lib.MTC_NORM_LAYER, mode != "post", mode == "post"
+    d = _lib.BlockNormDesc(rows=1, A=A, dtype=_lib.MTC_F32, has_branch=int(branch is not None), residual_scale=1.0, branch_scale=1.0,
+                           post_eps=1e-5, pre_eps=1e-5, post_kind=layer if post else 0, pre_kind=layer if pre else 0, ld_residual=A,
+                           ld_branch=A, ld_hidden=A, ld_normed=A)
+    weights = (_p(w if post else None), _p(b if post else None), _p(w if pre else None), _p(b if pre else None))
+    _lib.check(lib.mtc_block_norm_fwd(C.byref(d), _p(res), _p(branch), None, *weights, _p(hidden if branch is not None else None),
+                                      _p(normed if pre else None), _p(stats), _stream()))
+    ws = torch.empty(lib.mtc_block_norm_bwd_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=DEV)
+    _lib.check(lib.mtc_block_norm_bwd(C.byref(d), _p(res), _p(branch), None, *weights, _p(stats), _p(one if mode == "post" else None), A,
+                                      _p(one if pre else None), A, None, None, None, _p(dw if post else None), None,
+                                      _p(dw if pre else None), None, _p(ws), ws.numel(), _stream()))
+    v = (x if mode != "pair" else x + y).double()[0]                     # the fp32 sum, as the forward took it
+    mu, rstd = (stats[0, 0], stats[0, 1]) if post else (stats[0, 2], stats[0, 3])
+    u = (v - mu.double()) * rstd.double()
+    bad = (dw.double() - u).abs() > 2 * 2.0 ** -24 * 1.01 * u.abs()
+    assert not bool(bad.any()), (int(bad.sum()), float((dw.double() - u).abs().max()))
