@@ -102,3 +102,20 @@ def test_results_layout(tmp_path):
     assert list(sd) == ["b_enc", "W_enc", "W_dec", "b_dec", "threshold"]
     assert sd["W_enc"].shape == (32, 256) and sd["W_enc"].is_contiguous() and sd["W_enc"].dtype == torch.bfloat16
     assert r.list_experiments()["gpt2-small"][8][0]["has_final_checkpoint"]
+
+
+def test_make_needs_no_torch(tmp_path):
+    """libmtc.so is a C library: without a Python that has torch, `make` builds it alone; with one, the tensor binding too."""
+    import subprocess
+    import sys
+    fake = tmp_path / "python-without-torch"
+    fake.write_text(f'#!/bin/sh\nexec {sys.executable} -I -S "$@"\n')
+    fake.chmod(0o755)
+    none = tmp_path / "no-python"
+    plan = {}
+    for name, python in (("bare", fake), ("absent", none), ("torch", sys.executable)):
+        run = subprocess.run(["make", "-n", "-B", "-C", ROOT, f"PYTHON={python}"], capture_output=True, text=True, timeout=120)
+        assert run.returncode == 0, run.stderr
+        plan[name] = run.stdout
+    for name in plan:
+        assert "libmtc.so" in plan[name] and ("_torch_binding.so" in plan[name].replace("_torch_binding.so is left out", "")) == (name == "torch")
