@@ -56,9 +56,13 @@ class FusedAdam(torch.optim.Optimizer):
     `transcoder.make_decoder_weights_and_grad_unit_norm()` like the reference loop does;
     `step(project=True)` fuses that projection into the W_dec update (one pass over W_dec).
 
-    max_grad_norm: clip the gradients' common 2-norm to it (grad_clip.py) before the projection and the update; the
+    max_grad_norm: clip by the common 2-norm of the transcoder's own `.grad` tensors as `step()` finds them (grad_clip.py); the
     coefficient is applied as the gradients are read, with the bits that clipping them in place first would give, and the
-    `.grad` tensors stay as they are.  `last_grad_norm` then holds the norm before clipping (float32 scalar on the GPU).
+    `.grad` tensors stay as they are.  With `train_step` and `step(project=True)` that is before the projection; a caller who has
+    projected first (`make_decoder_weights_and_grad_unit_norm()`, then `step()`) gets the norm of the projected gradients, which is
+    smaller.  Parameters that other optimizers own (the norms and the gate of a spliced block) do not count and are not
+    clipped: use `clip_grad_norm_(block.parameters(), ...)` there instead.  `last_grad_norm` then holds the norm before clipping
+    (float32 scalar on the GPU; None after a step without gradients).
     `train_step` materialises the gradients in that case: their norm has to be known before the first parameter moves."""
 
     def __init__(self, transcoder, lr=3e-4, betas=(0.9, 0.99), eps=1e-8, max_grad_norm: Optional[float] = None):

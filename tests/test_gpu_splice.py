@@ -317,3 +317,20 @@ def test_a_backward_after_the_parameters_moved_is_refused(how):
     opt.zero_grad()
     m.reconstruct(x).sum().backward()                                    # the next forward and backward are as ever
     assert m.W_dec.grad is not None
+
+
+def test_the_optimizer_s_limit_is_the_transcoder_s_alone():
+    """FusedAdam(max_grad_norm) in a spliced block: the norms and the gate are not in its norm and stay as they are."""
+    from matryoshka_transcoder_amd.grad_clip import global_norm
+    b = _block(torch.float32, False, "rms", "channel", 31)
+    opt = FusedAdam(b.transcoder, max_grad_norm=1e-3)
+    x, a = (torch.randn(16, 64, generator=torch.Generator("cpu").manual_seed(s)).to(DEV) for s in (32, 33))
+    b(x, a).square().mean().backward()
+    own = global_norm([p.grad for p in b.transcoder.parameters()])
+    every = global_norm([p.grad for p in b.parameters() if p.grad is not None])
+    rest = {n: (p.detach().clone(), p.grad.clone()) for n, p in b.named_parameters() if not n.startswith("transcoder.")}
+    opt.step(project=True)
+    assert torch.equal(opt.last_grad_norm, own) and float(every) > float(own) > 1e-3
+    for n, p in b.named_parameters():
+        if n in rest:
+            assert torch.equal(p, rest[n][0]) and torch.equal(p.grad, rest[n][1])
