@@ -535,3 +535,47 @@ def test_backward_of_layer_norms_far_from_zero(mode, A):
     u = (v - mu.double()) * rstd.double()
     bad = (dw.double() - u).abs() > 2 * 2.0 ** -24 * 1.01 * u.abs()
     assert not bool(bad.any()), (int(bad.sum()), float((dw.double() - u).abs().max()))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("A", [8192, 7001])
+@pytest.mark.parametrize("kind,gate", [("rms", "none"), ("rms", "channel"), ("rms", "full"), ("layer", "none"), ("layer", "token"),
+                                       ("layer", "channel"), ("layer", "full")])
+def test_wide_rows_walked_more_than_once(kind, gate, A, dt):
+    """Above 6144 columns a row takes the whole workgroup of the backward: several rows each, so that the walk, the alternation
+    of the reduction's buffers and the column sums over rows repeat."""
+    _check(700 if A == 8192 else 600, A, dt, "pair", kind, kind, gate, rs=0.5 if gate == "token" else 1.0, seed=4)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("mode,post,pre", [("pre", None, "layer"), ("post", "layer", None), ("post", "rms", None), ("pair", None, "layer")])
+def test_wide_rows_of_single_modes(mode, post, pre, dt):
+    _check(600, 8192, dt, mode, post, pre, "none", seed=5)
+    _check(520, 6145, dt, mode, post, pre, "none", seed=6)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_streaming_with_all_column_sums(dt):
+    """Layer norms with biases beyond the Infinity Cache: every weight's and bias's gradient, and the rows as in blocks within it."""
+    g = torch.Generator("cpu").manual_seed(28)
+    rows, A = (26000, 2304) if dt == torch.bfloat16 else (13000, 2304)
+    gen = torch.Generator(DEV).manual_seed(28)
+    res, br, dh, dn = (torch.randn(rows, A, generator=gen, device=DEV).to(dt) for _ in range(4))
+    post, pre = _norm_module(g, A, "layer", dt), _norm_module(g, A, "layer", dt)
+    gate = _gate(g, "channel", rows, A, dt).requires_grad_(True)
+    names = ("gate", "post_w", "post_b", "pre_w", "pre_b")
+    leaves = [gate, post.weight, post.bias, pre.weight, pre.bias]
+
+    def both(lo, hi):
+        r, b = res[lo:hi].detach().requires_grad_(True), br[lo:hi].detach().requires_grad_(True)
+        out = residual_block_norm(r, b, post, gate=gate, pre=pre)
+        return list(out) + list(torch.autograd.grad(out, [r, b] + leaves, [dh[lo:hi], dn[lo:hi]]))
+
+    whole = both(0, rows)
+    for lo in range(0, rows, 4000):
+        part = both(lo, min(rows, lo + 4000))
+        for a, b in zip(whole[:4], part[:4]):
+            assert torch.equal(a[lo:lo + 4000], b)
+    want = N.reference(res, br, gate, _spec(post), _spec(pre), 1.0, 1.0, dh, dn)
+    for k, v in zip(names, whole[4:]):
+        N.compare(k, v, want[k], dt)
