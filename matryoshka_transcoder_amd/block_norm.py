@@ -98,7 +98,8 @@ def residual_block_norm(residual: torch.Tensor, branch: torch.Tensor, post: Opti
     block) returns `(hidden, pre(hidden))` from the same pass, the norm taken of the sum before its rounding.
 
     residual and branch: one shape [..., width], one dtype (float32 or bfloat16), one GPU; leading dimensions may be strided
-    or expanded.  gate: a scalar tensor, [width] (per channel), [..., 1] (per token) or the full shape.
+    or expanded.  gate: a scalar tensor, [width] (per channel), [..., 1] (per token) or the full shape; it multiplies, so an infinity or
+    NaN in the branch outlives a gate of 0.
     Differentiable in residual, branch, gate and both norms' parameters, once: a backward with create_graph = True raises, and
     so do forward-mode tangents, tracing (torch.jit.trace, make_fx) and a backward recorded into a HIP graph while an eager graph of
     the same leaves is alive."""

@@ -319,8 +319,8 @@ __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
 // row costs besides its elements (addresses, reductions) is paid once per row instead of once per wave and row.  A lane holds
 // NU units of 16 bytes, the wave's accesses are contiguous.  Every row is a wave of its own, dispatched in order, so that the
 // rows in flight are neighbours in memory.  Against the row group kernel above: 65536 x 2304 bf16 norm alone 97 against
-// 108 us (6.2 TB/s), 32768 x 2304 pair 98 against 115, 16384 x 2304 fp32 pair 100 against 112, 4096 x 2304 bf16 pair called in
-// a row 12.3 against 13.3.
+// 108 us (6.2 TB/s), 16384 x 2304 bf16 pair 51 against 58, fp32 102 against 110, 4096 x 2304 bf16 pair called in
+// a row 12.3 against 13.3 (with inputs that no cache holds 18.9 against 17.4).
 //   PLAIN: no bias and no gate per channel or element, which saves the registers of two rows.
 template <int DT, int NU> struct WaveRow {
     static constexpr int E = DType<DT>::kVec;
@@ -493,10 +493,14 @@ __global__ __launch_bounds__(256, (BRANCH && NU <= 5 ? 4 : 1)) void block_norm_w
 // and the column sums (over rows) X1 = gate D u_p, X2 = gate D, X3 = g u, X4 = g, from which block_norm_cols_kernel makes the
 // gradients of the weights, biases and the channel gate.  Each workgroup leaves one partial per column, summed in a
 // fixed order afterwards: no atomics, the same bits on every run.
-// One workgroup per CU of up to 768 threads (168 registers each, so that the column sums, the weights and two rows' operands fit),
-// several row groups in it where rows are short; its groups' sums meet in LDS.  Bound by memory at large sizes: 16384 x 4608 bf16
-// pair with a channel gate 163 us with the column kernel (5.6 TB/s over its six operands), 16384 x 2304 83 us (5.5); by the
-// operands' latency at small ones: 1024 x 2304 15 us.  A third row's operands in flight spill: 16384 x 1600 fp32 115 -> 167 us.
+// One workgroup per CU of up to 768 threads, several row groups in it where rows are short; its groups' sums meet in LDS.  168
+// registers each hold the column sums, the weights and two rows' operands (fp32 pairs with a gate per element and biases spill 24).
+// Rows above 6144 columns take up to 1024 threads with 128 registers: one row's operands, no prefetch, and pairs that keep
+// all four sums spill 8 to 45 registers, but for aligned bf16 ones without a gate per element.  Bound by memory at large sizes:
+// 16384 x 4608 bf16 pair with a channel gate 162 us with the column kernel (5.6 TB/s over its six operands), 16384 x 2304 84 us (5.4);
+// by the operands' latency at small ones (1024 x 2304 15 us, 4096 x 2304 30) and without prefetch: 4096 x 8192 bf16 RMS pair 87 us
+// (4.6 TB/s), layer norms 98, 4096 x 8191 in single elements 141.  A third row's operands in flight spill: 16384 x 1600 fp32
+// 115 -> 167 us.
 template <typename COLS, bool FULL> struct BwdRow {
     typename COLS::Raw branch, gate[FULL ? 1 : 0], d_hidden, residual, d_normed;
     uint32_t gr;
@@ -829,8 +833,11 @@ template <int DT, bool VEC, bool STREAM> static void launch_norm_fwd(const NormA
 }
 
 // What a wave can hold: 9 units a lane for a norm alone; with a branch 40 floats of a row, 36 where biases or a gate per
-// channel or element need rows of their own.  Beyond, the row group kernel is faster (4096 x 4608 bf16 pair 30 against
-// 47 us, 16384 x 2304 bf16 layer norms with a channel gate 65 against 78).
+// channel or element need rows of their own.  Row groups against one wave per row, us:
+//   beyond: bf16 pair 3584 wide 23.6 / 27.3 (4096 rows), 77.6 / 78.7 (16384); 4608 wide 29.9 / 33.7, 97.0 / 100.2; bf16 layer norms with a
+//           channel gate 2304 wide 19.5 / 26.4, 65.0 / 77.6
+//   within: bf16 pair 2304 wide 57.6 / 51.0 (16384 rows); fp32 1600 wide 76.9 / 71.1, 2304 wide 110 / 102, with layer norms 116 / 101.  Only
+//           around 4096 rows, read from memory, are row groups ahead by up to 2.5 us (17.4 / 18.9, fp32 layer norms 32.7 / 35.2)
 template <int DT, bool BRANCH, bool PLAIN> constexpr int wave_units() {
     return !BRANCH ? 9 : std::min(9, (PLAIN ? 40 : 36) / DType<DT>::kVec);
 }
@@ -893,9 +900,14 @@ extern "C" int mtc_block_norm_fwd(const mtc_block_norm_desc* d, const void* resi
                      row_vec(normed, d->ld_normed, d->rows, d->dtype);
     a.groups = a.T >= 256 ? 1 : 256 / a.T;
     // operands read and written once; beyond the Infinity Cache non-temporal accesses and, for two RMS norms (whose rows wait
-    // least), few waves that keep to few DRAM pages are faster: 16384 x 4608 bf16 pair 99 against 118 us.  Within the cache the
+    // least), few waves that keep to few DRAM pages are faster: 16384 x 4608 bf16 pair 97 against 118 us.  Within the cache the
     // opposite holds: 4096 x 2304 pair 14.8 against 17.0 us, and what follows finds plain stores in the cache (four such
-    // calls in a row 60 against 65 us).
+    // calls in a row 60 against 65 us).  12 / 20 / 28 waves per CU, us:
+    //   beyond, RMS:   16384 x 4608 bf16 97 / 113 / 108, 16384 x 4096 fp32 179 / 181 / 190, 65536 x 1001 bf16 111 / 117 / 120
+    //   beyond, layer: 16384 x 4608 bf16 134 / 116 / 116, 65536 x 1001 bf16 124 / 122 / 124, 32768 x 2304 bf16 127 / 130 / 129; 16384 x 4096 fp32
+    //                  183 / 186 / 197, where 28 is 7 % behind
+    //   within:        4096 x 4608 bf16 30.0 / 30.1 / 31.9, 1024 x 4608 10.9 / 10.5 / 10.5, 8192 x 1001 19.5 / 18.6 / 20.1
+    // Above 6144 columns a row takes 13 waves or more, and all three mean one workgroup per CU.
     const int passes = (branch ? 2 : 1) + (d->gate_kind == MTC_GATE_FULL) + (hidden != nullptr) + (normed != nullptr);
     a.streaming = d->rows * d->A * norm_elem(d->dtype) * passes > NORM_STREAM_BYTES;
     const bool layer = d->post_kind == MTC_NORM_LAYER || d->pre_kind == MTC_NORM_LAYER;
@@ -937,6 +949,8 @@ static void launch_norm_bwd_sums(const NormArgs& a, int sums, unsigned grid, hip
 template <int DT, bool VEC, bool BRANCH, bool PRE, bool FULL>
 static void launch_norm_bwd(const NormArgs& a, int sums, bool streaming, unsigned grid, hipStream_t s) {
     if (a.T * a.groups > NORM_BWD_T) launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, false, 1024, false>(a, sums, grid, s);
+    // gates per element have no streaming instance: beyond the cache that costs 8 % (16384 x 2304 fp32 pair 233 against 215 us, bf16
+    // 118 against 108), within it nothing
     else if (VEC && !FULL && streaming) launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, VEC, NORM_BWD_T, VEC && !FULL>(a, sums, grid, s);
     else launch_norm_bwd_sums<DT, VEC, BRANCH, PRE, FULL, VEC, NORM_BWD_T, false>(a, sums, grid, s);
 }
