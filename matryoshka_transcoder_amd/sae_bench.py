@@ -138,7 +138,9 @@ class MatryoshkaAutoInterpAdapter(MatryoshkaTranscoder):
     """`MatryoshkaTranscoder` + the attributes SAEBench expects on an SAE (wrappers.py:53-109).
 
     A run trained with cfg["source_norm"] saw the norm of what its hook yields: the adapter keeps a frozen copy of that norm
-    (`source_norm`, not among its parameters: the state_dict stays the reference's) and applies it to every source it is given."""
+    (`source_norm`, not among its parameters: the state_dict stays the reference's) and applies it to every source it is given.
+    Give it what its hook yields, not the batches of a store with the same source_norm, which are normed already (for those: a
+    MatryoshkaTranscoder, or cfg["source_norm"] = None)."""
 
     def __init__(self, cfg: dict, *, sae_cfg: AutoInterpSAEConfig) -> None:
         own = copy.deepcopy(dict(cfg))
