@@ -9,17 +9,17 @@ LIB   := matryoshka_transcoder_amd/libmtc.so
 FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
 
 # host side of the block norms and the gradient clipping on torch tensors (no kernels; calls libmtc.so by address).  Built where
-# PYTHON has torch; libmtc.so itself, and whoever calls it from C, does without
+# PYTHON has a ROCm torch; libmtc.so itself, and whoever calls it from C, does without
 BINDING := matryoshka_transcoder_amd/_torch_binding.so
 PYTHON  ?= python3
 TORCH   := $(shell $(PYTHON) -c "import importlib.util as u; s = u.find_spec('torch'); print(s.submodule_search_locations[0] if s else '')" 2>/dev/null)
 PYINC    = $(shell $(PYTHON) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
-ifneq ($(TORCH),)
+ifneq ($(wildcard $(TORCH)/lib/libc10_hip.so),)
 all: $(LIB) $(BINDING)
 else
 all: $(LIB)
-	@echo "no torch for $(PYTHON): _torch_binding.so is left out"
+	@echo "no ROCm torch for $(PYTHON): _torch_binding.so is left out"
 endif
 
 $(BINDING): $(CSRC)/torch_binding.cpp include/mtc.h

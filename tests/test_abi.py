@@ -111,9 +111,12 @@ def test_make_needs_no_torch(tmp_path):
     fake = tmp_path / "python-without-torch"
     fake.write_text(f'#!/bin/sh\nexec {sys.executable} -I -S "$@"\n')
     fake.chmod(0o755)
-    none = tmp_path / "no-python"
+    other = tmp_path / "python-with-another-torch"                          # found, but not built for ROCm
+    (tmp_path / "torch" / "lib").mkdir(parents=True)
+    other.write_text(f'#!/bin/sh\necho {tmp_path / "torch"}\n')
+    other.chmod(0o755)
     plan = {}
-    for name, python in (("bare", fake), ("absent", none), ("torch", sys.executable)):
+    for name, python in (("bare", fake), ("other", other), ("absent", tmp_path / "no-python"), ("torch", sys.executable)):
         run = subprocess.run(["make", "-n", "-B", "-C", ROOT, f"PYTHON={python}"], capture_output=True, text=True, timeout=120)
         assert run.returncode == 0, run.stderr
         plan[name] = run.stdout
