@@ -66,8 +66,9 @@ class TranscoderActivationsStore:
     def __init__(self, model, cfg: dict, source=None, token_iterator: Optional[Iterator] = None):
         """cfg["source_norm"] (optional, a block_norm.BlockNorm on the GPU): the harvested source is the residual stream in
         front of a block, and the block's own norm of it becomes the transcoder's source activation -- one stream to
-        harvest or store instead of two, for models that have no hook behind that norm.  cfg["source_hook_point"] then has to
-        be a point in front of the norm, and the model has to expose it: what a norm has left already is refused."""
+        harvest or store instead of two, for models that have no hook behind that norm.  Harvesting from a
+        model, cfg["source_hook_point"] then has to be a point in front of the norm, and the model has to expose it: what a norm
+        has left already is refused."""
         self.model = model
         self.source_norm = cfg.get("source_norm")
         if self.source_norm is not None and not isinstance(self.source_norm, torch.nn.Module):
@@ -75,7 +76,7 @@ class TranscoderActivationsStore:
         self.config = cfg
         self.device = cfg["device"]
         self.source_hook_point = cfg.get("source_hook_point")
-        if self.source_norm is not None and str(self.source_hook_point).endswith("hook_normalized"):
+        if self.source_norm is not None and source is None and str(self.source_hook_point).endswith("hook_normalized"):
             raise _lib.MtcError(f"cfg['source_norm'] norms the residual stream, but {self.source_hook_point} (hook_normalized) lies "
                                 "behind a norm")
         self.target_hook_point = cfg.get("target_hook_point")

@@ -58,6 +58,11 @@ def test_a_source_point_behind_the_norm_is_refused():
     with pytest.raises(_lib.MtcError, match="hook_normalized"):
         _store(_Model(), _Doubling(), "blocks.0.ln2.hook_normalized")
     _store(_Model(), None, "blocks.0.ln2.hook_normalized")                   # without a source norm it is a point like any other
+    from matryoshka_transcoder_amd.activation_store import TensorPairSource
+    cfg = dict(act_size=8, batch_size=4, num_batches_in_buffer=1, device="cpu", dtype=torch.float32, source_norm=_Doubling(),
+               source_hook_point="blocks.0.ln2.hook_normalized")
+    store = TranscoderActivationsStore(None, cfg, source=TensorPairSource([(torch.ones(4, 8), torch.ones(4, 8))]))
+    assert torch.equal(store.next_batch()[0], torch.full((4, 8), 2.0))       # rows that are handed over are residual rows, whatever the name
 
 
 # ---------------------------------------------------------------- a saved run keeps its norm, an adapter takes it along
